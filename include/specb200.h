@@ -264,6 +264,45 @@ int specb200_attention(int dtype, const void* q, const void* k_pool, const void*
                        int n_kv_heads, int head_dim, int max_kv_len, float scale, void* out,
                        void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
 
+/* ======================================================================================
+ * 8-bit linears: e4m3 operands with an fp32 scale for each group of 128 (no counterpart in
+ * the reference, which has none). An e4m3 value q stands for q * s with its group's scale
+ *   s = max(max |y| over the group, 2^-100) / 448,   q = e4m3(y / s), nearest even.
+ * Activations [M, K] have a scale per row and 128 columns: scales [M, ceil(K / 128)] fp32.
+ * Weights [N, K] have one per 128 x 128 block: [ceil(N / 128), ceil(K / 128)]. The last groups
+ * may be short. Row pitches (ld*) count elements; any pitch and alignment is accepted except
+ * where a function says otherwise, rows on 16-byte boundaries are faster. A NaN in a group
+ * makes its values and scale NaN, an infinity makes the scale infinite. Nothing is written
+ * behind a row's last element. Outputs must not overlap inputs unless a function says so.
+ * M = 0 is a no-op. No workspaces: calls on any streams may overlap.
+ * ====================================================================================== */
+
+/* block_rows 1: a scale per row and 128 columns; 128: per 128 x 128 block. x: [M, K] of `dtype`. */
+int specb200_quantize_fp8(int dtype, const void* x, int64_t ldx, int M, int K, int block_rows, void* q,
+                          int64_t ldq, float* scales, void* stream);
+
+/* RMSNorm with the residual update in front and an 8-bit output:
+ *   h = T(x + delta) (delta NULL: h = x, not stored; h may be x or delta),
+ *   y = weight * h / sqrt(mean(h^2) + eps) in fp32, (q, scales) = quantized y.
+ * H <= 32768 (SPECB200_ERR_UNSUPPORTED beyond). */
+int specb200_rmsnorm_fp8(int dtype, const void* x, int64_t ldx, const void* delta, int64_t ldd, const void* weight,
+                         int M, int H, float eps, void* h, int64_t ldh, void* q, int64_t ldq, float* scales,
+                         void* stream);
+
+/* (q, scales) = quantized silu(gate) * up, fp32 in between. gate_up: [M, 2 I], the gate columns
+ * then the up columns, or with `packed` 64-column groups of gate then up (the row order of
+ * specb200_layer_weights.w_gate_up; I % 64 == 0). */
+int specb200_silu_mul_fp8(int dtype, const void* gate_up, int64_t ld, int M, int I, int packed, void* q,
+                          int64_t ldq, float* scales, void* stream);
+
+/* y[m, n] = sum_b x_scales[m, b] * w_scales[n / 128, b] * sum_{k in group b} x[m, k] * w[n, k] on
+ * the tensor cores, accumulated in fp32. x [M, K], w [N, K] e4m3: bases on 16-byte boundaries,
+ * pitches multiples of 16. y: fp32 (out_f32) or bf16. Results do not depend on scheduling.
+ * status: device int32, or NULL; cleared by the call, set if a device-side wait gave up. */
+int specb200_linear_fp8(const void* x, int64_t ldx, const float* x_scales, const void* w, int64_t ldw,
+                        const float* w_scales, int M, int N, int K, int out_f32, void* y, int64_t ldy,
+                        int32_t* status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

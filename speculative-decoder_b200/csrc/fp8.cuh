@@ -1,0 +1,35 @@
+// 8-bit operands with scales: an e4m3 value q stands for q * s, where s is the fp32 scale of its
+// group. Activations [M, K] have one scale per row and 128 columns, weights [N, K] one per
+// 128 x 128 block; the last groups of a row or column may be short.
+//   s = max(max |y| over the group, 2^-100) / 448,   q = e4m3(y / s)
+// 448 is e4m3's largest value. The floor keeps 1 / s finite for groups of zeros; a NaN or an
+// infinity in a group makes its scale NaN or infinite and so stays visible in every product.
+#pragma once
+#include <cuda_fp8.h>
+
+#include "common.cuh"
+
+namespace specb200 {
+
+constexpr int kFp8Group = 128;
+constexpr float kE4m3Max = 448.f;
+constexpr float kFp8MinAmax = 7.888609052210118e-31f;  // 2^-100
+
+// Magnitudes are compared as the bit patterns of |x|: the order of the values, with every NaN
+// above infinity, so a NaN wins the maximum instead of being dropped by fmaxf.
+SPECB200_DEVINL uint32_t mag_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+SPECB200_DEVINL float floor_amax(float amax) { return amax < kFp8MinAmax ? kFp8MinAmax : amax; }
+
+// Eight fp32 values as e4m3, rounded to nearest even; finite values beyond 448 (a group's
+// maximum can exceed it by an ulp) saturate, NaN stays NaN.
+SPECB200_DEVINL uint2 pack_e4m3(const float (&f)[8]) {
+  uint32_t h[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    h[i] = __nv_cvt_float2_to_fp8x2(make_float2(f[2 * i], f[2 * i + 1]), __NV_SATFINITE, __NV_E4M3);
+  return make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
+}
+
+inline bool fp8_aligned(const void* p, uint64_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+
+}  // namespace specb200

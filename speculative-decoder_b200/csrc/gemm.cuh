@@ -79,5 +79,8 @@ int launch_gemm_simt(const GemmShape& s, const T* w, const T* x, const Epilogue&
 // TMA descriptor helpers (forward.cu / gemm.cu).
 bool make_tmap_bf16_2d(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer, uint32_t box_inner,
                        uint32_t box_outer);
+// The same over bytes (e4m3 operands), rows `pitch` bytes apart.
+bool make_tmap_u8_2d(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer, uint64_t pitch,
+                     uint32_t box_inner, uint32_t box_outer);
 
 }  // namespace specb200

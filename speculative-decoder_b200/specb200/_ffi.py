@@ -10,6 +10,7 @@ library or without a CUDA device every entry point raises.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from pathlib import Path
 
@@ -82,6 +83,14 @@ PROTOTYPES: dict[str, tuple] = {
     "specb200_attention": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p,
                                    c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p, c_void_p, c_size_t,
                                    c_void_p, c_void_p]),
+    "specb200_quantize_fp8": (c_int, [c_int, c_void_p, c_int64, c_int, c_int, c_int, c_void_p, c_int64, c_void_p,
+                                      c_void_p]),
+    "specb200_rmsnorm_fp8": (c_int, [c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_int, c_float,
+                                     c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p]),
+    "specb200_silu_mul_fp8": (c_int, [c_int, c_void_p, c_int64, c_int, c_int, c_int, c_void_p, c_int64, c_void_p,
+                                      c_void_p]),
+    "specb200_linear_fp8": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int, c_int, c_int,
+                                    c_int, c_void_p, c_int64, c_void_p, c_void_p]),
 }
 
 _lib: ctypes.CDLL | None = None
@@ -151,6 +160,14 @@ def ptr(t: torch.Tensor | None) -> int | None:
 
 def stream_ptr(device: torch.device | None = None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+_HERE = contextlib.nullcontext()
+
+
+def on_device(device: torch.device):
+    """Makes `device` current for a launch (a stream takes launches from its own device only)."""
+    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 class Workspace:

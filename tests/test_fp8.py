@@ -1,0 +1,617 @@
+"""The 8-bit operators (quantize_fp8, rmsnorm_fp8, silu_mul_fp8, linear_fp8) against their formulas
+in 64 bits, and their refusals.
+
+Tolerances, with u = 2^-24 (half a step of fp32):
+- scales: the roundings of the fp32 steps that form them, counted per operator;
+- quantized values: e4m3 of the 64-bit quotient y / s moved down and up by the relative error d
+  that fp32 leaves in it; the kernel's value lies between the two, so any value is exact unless the
+  quotient is within d of the middle between two e4m3 numbers;
+- products: fp32 accumulation with truncation, a step of 2^-23 of the group's sum of |x w| for each
+  of its 128 terms and 4 instructions, then u for each group, split and scale factor, then the
+  output's own half step.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+U = 2.0 ** -24
+FLOOR = 2.0 ** -100
+DEV = "cuda"
+BF16, F32 = torch.bfloat16, torch.float32
+F8 = torch.float8_e4m3fn
+
+
+def _ops():
+    from specb200 import ops
+
+    return ops
+
+
+def _lib():
+    from specb200 import _ffi
+
+    return _ffi.lib()
+
+
+def _rand(seed, *shape, dtype=F32, spread=0.8):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(*shape, generator=g) * torch.exp(spread * torch.randn(shape[-1], generator=g))
+    return x.to(DEV, dtype)
+
+
+def _amax(y, block_rows=1):
+    """Largest |y| of each group of 128 columns x block_rows rows, of fp64 rows [M, K]."""
+    m, k = y.shape
+    y = torch.nn.functional.pad(y.abs(), (0, -k % 128, 0, -m % block_rows))
+    return y.reshape(y.shape[0] // block_rows, block_rows, -1, 128).amax(dim=(1, 3))
+
+
+def _spread(s, m, k, block_rows=1):
+    """Scales [blocks, groups] as one per element [M, K]."""
+    return s.repeat_interleave(block_rows, 0)[:m].repeat_interleave(128, 1)[:, :k]
+
+
+def _check_quantized(q, s, y64, d, s_tol, block_rows=1):
+    """q, s as the quantization of the exact rows y64; d: relative error of y / s in fp32."""
+    m, k = y64.shape
+    want = _amax(y64, block_rows).clamp_min(FLOOR) / 448
+    assert s.dtype == F32 and s.shape == want.shape
+    assert ((s.double() - want).abs() <= s_tol * want).all()
+    t = y64 / _spread(want, m, k, block_rows)
+    a, b = (t * (1 - d)).to(F8).float(), (t * (1 + d)).to(F8).float()
+    got = q.float()
+    assert q.dtype == F8 and got.shape == t.shape
+    assert ((got >= torch.minimum(a, b)) & (got <= torch.maximum(a, b))).all()
+
+
+def _operands(seed, m, n, k):
+    """Random e4m3 operands with scales of their own, independent of the engine's quantizers."""
+    g = torch.Generator().manual_seed(seed)
+    groups = -(-k // 128)
+
+    def rows(r):
+        held = torch.zeros(r, (k + 15) // 16 * 16, dtype=torch.uint8)
+        held[:, :k] = (torch.randn(r, k, generator=g) * 60).clamp(-448, 448).to(F8).view(torch.uint8)
+        return held.to(DEV).view(F8)[:, :k]
+
+    x, w = rows(m), rows(n)
+    xs = torch.exp(torch.randn(m, groups, generator=g)).to(DEV) * 1e-2
+    ws = torch.exp(torch.randn(-(-n // 128), groups, generator=g)).to(DEV) * 1e-3
+    return x, xs, w, ws
+
+
+def _product64(x, xs, w, ws):
+    """(y, sum of |terms|) in fp64."""
+    m, k = x.shape
+    n = w.shape[0]
+    a = x.double() * _spread(xs.double(), m, k)
+    b = w.double() * _spread(ws.double(), n, k, 128)
+    return a @ b.T, a.abs() @ b.abs().T
+
+
+def _check_product(y, x, xs, w, ws, out_f32):
+    want, mag = _product64(x, xs, w, ws)
+    groups = xs.shape[-1]
+    tol = mag * (132 * 2.0 ** -23 + (groups + 8 + 3) * U)
+    if not out_f32:
+        tol = tol + (want.abs() + tol) * 2.0 ** -8
+    assert y.dtype == (F32 if out_f32 else BF16) and y.shape == want.shape
+    err = (y.double() - want).abs()
+    assert (err <= tol).all(), f"worst error / tolerance {(err / tol.clamp_min(1e-300)).max().item():.3g}"
+
+
+# ---------------------------------------------------------------- refusals, on the host
+def _buf(nbytes=4096, offset=0):
+    """A host address that the argument checks may look at (the calls below are refused before any launch)."""
+    raw = (ctypes.c_char * (nbytes + 64))()
+    base = (ctypes.addressof(raw) + 15) // 16 * 16
+    return raw, base + offset
+
+
+def test_quantize_refuses_bad_arguments_on_the_host():
+    from specb200 import _ffi
+
+    lib = _lib()
+    keep, p = _buf()
+    ok = dict(dtype=_ffi.BF16, x=p, ldx=64, M=2, K=64, rows=1, q=p, ldq=64, s=p)
+    call = lambda **k: lib.specb200_quantize_fp8(*{**ok, **k}.values(), None)  # noqa: E731
+    for bad in (dict(M=-1), dict(K=0), dict(ldx=63), dict(ldq=63), dict(rows=2), dict(rows=64), dict(x=None),
+                dict(q=None), dict(s=None)):
+        assert call(**bad) == _ffi.ERR_ARG, bad
+        assert b"quantize_fp8" in lib.specb200_last_error()
+    assert call(dtype=2) == _ffi.ERR_UNSUPPORTED
+    assert call(M=0, x=None, q=None, s=None) == _ffi.OK
+    assert call(M=2 ** 31 - 1, K=2 ** 30, ldx=2 ** 30, ldq=2 ** 30) == _ffi.ERR_ARG
+
+
+def test_rmsnorm_refuses_bad_arguments_on_the_host():
+    from specb200 import _ffi
+
+    lib = _lib()
+    keep, p = _buf()
+    ok = dict(dtype=_ffi.F32, x=p, ldx=64, d=p, ldd=64, w=p, M=2, H=64, eps=1e-5, h=p, ldh=64, q=p, ldq=64, s=p)
+    call = lambda **k: lib.specb200_rmsnorm_fp8(*{**ok, **k}.values(), None)  # noqa: E731
+    for bad in (dict(M=-1), dict(H=0), dict(ldx=63), dict(ldd=63), dict(ldh=63), dict(ldq=63), dict(x=None),
+                dict(w=None), dict(h=None), dict(q=None), dict(s=None)):
+        assert call(**bad) == _ffi.ERR_ARG, bad
+    assert call(dtype=7) == _ffi.ERR_UNSUPPORTED
+    assert call(H=32769, ldx=40000, ldd=40000, ldh=40000, ldq=40000) == _ffi.ERR_UNSUPPORTED
+    assert call(M=0) == _ffi.OK
+
+
+def test_silu_mul_refuses_bad_arguments_on_the_host():
+    from specb200 import _ffi
+
+    lib = _lib()
+    keep, p = _buf()
+    ok = dict(dtype=_ffi.BF16, x=p, ld=128, M=2, I=64, packed=0, q=p, ldq=64, s=p)
+    call = lambda **k: lib.specb200_silu_mul_fp8(*{**ok, **k}.values(), None)  # noqa: E731
+    for bad in (dict(M=-1), dict(I=0), dict(ld=127), dict(ldq=63), dict(packed=1, I=32), dict(x=None), dict(q=None),
+                dict(s=None)):
+        assert call(**bad) == _ffi.ERR_ARG, bad
+    assert call(dtype=-1) == _ffi.ERR_UNSUPPORTED
+    assert call(M=0) == _ffi.OK
+
+
+def test_linear_refuses_bad_arguments_on_the_host():
+    from specb200 import _ffi
+
+    lib = _lib()
+    keep, p = _buf()
+    ok = dict(x=p, ldx=64, xs=p, w=p, ldw=64, ws=p, M=2, N=16, K=64, f32=0, y=p, ldy=16, status=None)
+    call = lambda **k: lib.specb200_linear_fp8(*{**ok, **k}.values(), None)  # noqa: E731
+    for bad in (dict(M=-1), dict(N=0), dict(K=0), dict(ldx=48), dict(ldw=48), dict(ldx=72), dict(ldw=72), dict(ldy=15),
+                dict(x=None), dict(xs=None), dict(w=None), dict(ws=None), dict(y=None), dict(x=p + 8), dict(w=p + 1)):
+        assert call(**bad) == _ffi.ERR_ARG, bad
+        assert b"linear_fp8" in lib.specb200_last_error()
+    assert call(M=0) == _ffi.OK
+
+
+def test_host_tensors_are_refused():
+    x = torch.zeros(2, 64)
+    for call in (lambda o: o.quantize_fp8(x), lambda o: o.rmsnorm_fp8(x, x[0], 1e-5), lambda o: o.silu_mul_fp8(x),
+                 lambda o: o.linear_fp8(x.to(F8), x, x.to(F8), x)):
+        with pytest.raises(RuntimeError, match="CUDA"):
+            call(_ops())
+
+
+@pytest.mark.gpu
+def test_wrappers_refuse_mismatched_tensors():
+    ops = _ops()
+    x = torch.zeros(4, 256, device=DEV, dtype=BF16)
+    with pytest.raises(NotImplementedError):
+        ops.quantize_fp8(x.half())
+    with pytest.raises(ValueError):
+        ops.quantize_fp8(x, block_rows=2)
+    with pytest.raises(ValueError):
+        ops.quantize_fp8(x.view(2, 2, 256), block_rows=128)
+    with pytest.raises(ValueError):
+        ops.quantize_fp8(x[:, :0])
+    with pytest.raises(ValueError):
+        ops.rmsnorm_fp8(x, x[0, :128], 1e-5)
+    with pytest.raises(ValueError):
+        ops.rmsnorm_fp8(x, x[0].float(), 1e-5)
+    with pytest.raises(ValueError):
+        ops.rmsnorm_fp8(x, x[0], 1e-5, delta=x[:2])
+    with pytest.raises(ValueError):
+        ops.rmsnorm_fp8(x, x[0].cpu(), 1e-5)
+    with pytest.raises(NotImplementedError):
+        ops.rmsnorm_fp8(torch.zeros(1, 32776, device=DEV), torch.ones(32776, device=DEV), 1e-5)
+    with pytest.raises(ValueError):
+        ops.silu_mul_fp8(x[:, :255])
+    with pytest.raises(ValueError):
+        ops.silu_mul_fp8(x[:, :192], packed=True)
+    q, s = ops.quantize_fp8(x)
+    w, ws = ops.quantize_fp8(torch.zeros(130, 256, device=DEV, dtype=BF16), block_rows=128)
+    for bad in ((x, s, w, ws), (q, s, x, ws), (q[:, :128], s, w, ws), (q, s[:, :1], w, ws), (q, s, w, ws[:1]),
+                (q, s.double(), w, ws), (q, s, w, ws.bfloat16()), (q, s.cpu(), w, ws), (q, s, w[0], ws)):
+        with pytest.raises(ValueError):
+            ops.linear_fp8(*bad)
+
+
+# ---------------------------------------------------------------- quantize
+SIZES = [(1, 1), (1, 16), (3, 127), (5, 128), (7, 129), (130, 576), (257, 2048), (129, 1000), (1, 8192)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("block_rows", [1, 128])
+@pytest.mark.parametrize("m,k", SIZES)
+def test_quantize(m, k, block_rows, dtype):
+    x = _rand(m * 7 + k, m, k, dtype=dtype)
+    q, s = _ops().quantize_fp8(x, block_rows=block_rows)
+    _check_quantized(q, s, x.double(), d=4 * U, s_tol=2 * U, block_rows=block_rows)  # 448/amax, product; amax/448
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("block_rows", [1, 128])
+def test_quantize_of_views(block_rows, dtype):
+    """Columns of a wider matrix (rows off any 16-byte boundary), every other row, a transposed view."""
+    wide = _rand(1, 60, 700, dtype=dtype)
+    for x in (wide[:, 1:301], wide[:, 8:264], wide[::2, 3:200], wide.t(), wide[0:1, 5:600]):
+        q, s = _ops().quantize_fp8(x, block_rows=block_rows)
+        _check_quantized(q, s, x.double(), d=4 * U, s_tol=2 * U, block_rows=block_rows)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("block_rows", [1, 128])
+def test_quantize_edge_values(block_rows):
+    """Groups of zeros, of values below the floor, near fp32's ends, and groups that hold a NaN or an infinity."""
+    x = _rand(2, 4, 128 * 7)
+    x[:, 0:128] = 0
+    x[:, 128:256] *= 1e-33
+    x[:, 256:384] *= 1e-38
+    x[:, 384:512] *= 1e36
+    x[2, 512] = float("nan")
+    x[1, 640] = float("inf")
+    q, s = _ops().quantize_fp8(x, block_rows=block_rows)
+    keep = [0, 1, 2, 3, 6]
+    cols = torch.cat([torch.arange(g * 128, g * 128 + 128) for g in keep]).to(DEV)
+    _check_quantized(q.float()[:, cols].to(F8), s[:, keep], x[:, cols].double(), d=4 * U, s_tol=2 * U,
+                     block_rows=block_rows)
+    qn, qi = q.float()[:, 512:640], q.float()[:, 640:768]
+    rows_n = [2] if block_rows == 1 else [0, 1, 2, 3]
+    rows_i = [1] if block_rows == 1 else [0, 1, 2, 3]
+    assert qn[rows_n].isnan().all() and s[rows_n if block_rows == 1 else 0, 4].isnan().all()
+    assert torch.isinf(s[rows_i if block_rows == 1 else 0, 5]).all() and qi[1, 0].isnan()
+    rest = qi[rows_i].clone()
+    rest[rows_i.index(1), 0] = 0
+    assert (rest == 0).all()
+
+
+@pytest.mark.gpu
+def test_rows_of_leading_dimensions():
+    ops = _ops()
+    x = _rand(3, 2, 3, 200, dtype=BF16)
+    q, s = ops.quantize_fp8(x)
+    q2, s2 = ops.quantize_fp8(x.view(6, 200))
+    assert q.shape == (2, 3, 200) and s.shape == (2, 3, 2)
+    assert torch.equal(q.float().view(6, 200), q2.float()) and torch.equal(s.view(6, 2), s2)
+    q1, s1 = ops.quantize_fp8(x[0, 0])
+    assert torch.equal(q1.float(), q2.float()[0]) and torch.equal(s1, s2[0])
+    w, ws = ops.quantize_fp8(_rand(4, 96, 200, dtype=BF16), block_rows=128)
+    y = ops.linear_fp8(q, s, w, ws)
+    assert y.shape == (2, 3, 96) and torch.equal(y.view(6, 96), ops.linear_fp8(q2, s2, w, ws))
+    assert torch.equal(ops.linear_fp8(q1, s1, w, ws), y[0, 0])
+
+
+@pytest.mark.gpu
+def test_no_rows():
+    ops = _ops()
+    x = torch.zeros(0, 200, device=DEV, dtype=BF16)
+    q, s = ops.quantize_fp8(x)
+    assert q.shape == (0, 200) and s.shape == (0, 2)
+    w, ws = ops.quantize_fp8(_rand(4, 96, 200, dtype=BF16), block_rows=128)
+    assert ops.linear_fp8(q, s, w, ws).shape == (0, 96)
+    q, s, h = ops.rmsnorm_fp8(x, x.new_ones(200), 1e-5, delta=x)
+    assert q.shape == (0, 200) and s.shape == (0, 2) and h.shape == (0, 200)
+    q, s = ops.silu_mul_fp8(x)
+    assert q.shape == (0, 100) and s.shape == (0, 1)
+    q, s = ops.quantize_fp8(torch.zeros(2, 0, 64, device=DEV))
+    assert q.shape == (2, 0, 64) and s.shape == (2, 0, 1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("op", ["rows", "blocks", "norm", "silu"])
+def test_nothing_is_written_outside_the_rows(op):
+    """Through the C ABI into buffers with a pitch and a frame of their own, at an odd offset."""
+    from specb200 import _ffi
+
+    lib = _lib()
+    m, k, pitch = 5, 201, 230
+    x = _rand(5, m, 2 * k, dtype=BF16)
+    weight = _rand(6, k, dtype=BF16)
+    q = torch.full((m + 2, pitch), 0x55, dtype=torch.uint8, device=DEV)
+    blocks = 1 if op == "blocks" else m
+    s = torch.full((blocks + 2, 2), -7.0, device=DEV)
+    h = torch.full((m + 2, pitch), 3.0, dtype=BF16, device=DEV)
+    qp, sp, hp = q[1].data_ptr() + 3, s[1].data_ptr(), h[1].data_ptr() + 2 * 5
+    st = torch.cuda.current_stream().cuda_stream
+    if op in ("rows", "blocks"):
+        rc = lib.specb200_quantize_fp8(_ffi.BF16, x.data_ptr(), 2 * k, m, k, 1 if op == "rows" else 128, qp, pitch, sp, st)
+    elif op == "norm":
+        rc = lib.specb200_rmsnorm_fp8(_ffi.BF16, x.data_ptr(), 2 * k, x.data_ptr() + 2 * k, 2 * k, weight.data_ptr(), m, k,
+                                      1e-5, hp, pitch, qp, pitch, sp, st)
+    else:
+        rc = lib.specb200_silu_mul_fp8(_ffi.BF16, x.data_ptr(), 2 * k, m, k, 0, qp, pitch, sp, st)
+    assert rc == 0, lib.specb200_last_error()
+    flat = q.flatten()
+    inside = torch.zeros_like(flat, dtype=torch.bool)
+    for r in range(m):
+        inside[pitch + 3 + r * pitch: pitch + 3 + r * pitch + k] = True
+    assert (flat[~inside] == 0x55).all() and (flat[inside] != 0x55).any()
+    assert (s[0] == -7).all() and (s[blocks + 1] == -7).all() and (s[1:blocks + 1] > 0).all()
+    if op == "norm":
+        flat = h.flatten()
+        inside = torch.zeros_like(flat, dtype=torch.bool)
+        for r in range(m):
+            inside[pitch + 5 + r * pitch: pitch + 5 + r * pitch + k] = True
+        assert (flat[~inside] == 3).all()
+        assert torch.equal(flat[inside].view(m, k), (x[:, :k].float() + x[:, k:].float()).to(BF16))
+
+
+# ---------------------------------------------------------------- RMSNorm
+# The sum of squares: at most 32 in a thread, 5 shuffles and 32 warps, so 69 roundings; half of
+# that in 1 / rms, then the mean, the sum with eps, the root, the quotient, w h, (w h) r and / 448.
+NORM_S = (69 / 2 + 7) * U
+
+
+def _norm64(h, weight, eps):
+    h = h.double()
+    return h * (h.square().mean(-1, keepdim=True) + eps).rsqrt() * weight.double()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("delta", [False, True])
+@pytest.mark.parametrize("m,k", SIZES + [(3, 8200), (2, 16392), (2, 32768), (700, 64)])
+def test_rmsnorm(m, k, delta, dtype):
+    x = _rand(m + 3 * k, m, k, dtype=dtype)
+    weight = (1 + 0.3 * _rand(k, k, spread=0.0)).to(dtype)
+    d = _rand(m + k, m, k, dtype=dtype) if delta else None
+    out = _ops().rmsnorm_fp8(x, weight, 1e-5, delta=d)
+    h = x
+    if delta:
+        h = (x.float() + d.float()).to(dtype)
+        assert torch.equal(out[2], h)
+    assert len(out) == (3 if delta else 2)
+    _check_quantized(out[0], out[1], _norm64(h, weight, 1e-5), d=4 * U, s_tol=NORM_S)  # w h, 448 / max, product
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_rmsnorm_of_views_and_in_place(dtype):
+    from specb200 import _ffi
+
+    lib = _lib()
+    wide = _rand(7, 20, 900, dtype=dtype)
+    weight = _rand(8, 300, dtype=dtype)
+    for x, d in ((wide[:, 1:301], wide[:, 401:701]), (wide[::2, 16:316], wide[::2, 320:620])):
+        q, s, h = _ops().rmsnorm_fp8(x, weight, 1e-6, delta=d)
+        want = (x.float() + d.float()).to(dtype)
+        assert torch.equal(h, want)
+        _check_quantized(q, s, _norm64(want, weight, 1e-6), d=4 * U, s_tol=NORM_S)
+    # the residual stream updated in its place (h = x)
+    m, k = 6, 300
+    x, d = wide[:m, :k].contiguous(), wide[:m, 400:400 + k].contiguous()
+    q, s, h = _ops().rmsnorm_fp8(x, weight, 1e-6, delta=d)
+    q2, s2 = torch.empty(m, k, dtype=torch.uint8, device=DEV), torch.empty_like(s)
+    rc = lib.specb200_rmsnorm_fp8(_ffi.BF16 if dtype == BF16 else _ffi.F32, x.data_ptr(), k, d.data_ptr(), k,
+                                  weight.data_ptr(), m, k, 1e-6, x.data_ptr(), k, q2.data_ptr(), k, s2.data_ptr(),
+                                  torch.cuda.current_stream().cuda_stream)
+    assert rc == 0 and torch.equal(x, h) and torch.equal(s2, s) and torch.equal(q2, q.contiguous().view(torch.uint8))
+
+
+@pytest.mark.gpu
+def test_rmsnorm_edge_rows():
+    """A row of zeros, rows so small that eps decides, groups under the floor, weights of zero, and
+    rows that hold a NaN or an infinity: each keeps to itself."""
+    k = 400
+    x = _rand(9, 8, k)
+    x[0] = 0
+    x[1] *= 1e-20
+    x[2, :128] *= 1e-36
+    x[3, :128] = 0
+    x[4, 7] = float("nan")
+    x[5, 7] = float("inf")
+    x[6] *= 1e15
+    weight = _rand(10, k)
+    weight[128:256] = 0
+    q, s = _ops().rmsnorm_fp8(x, weight, 1e-5)
+    ok = [0, 1, 2, 3, 6, 7]
+    _check_quantized(q.float()[ok].to(F8), s[ok], _norm64(x[ok], weight, 1e-5), d=NORM_S + 4 * U, s_tol=NORM_S)
+    assert s[4].isnan().all() and q.float()[4].isnan().all()
+    # 1 / rms is zero: finite elements give zero, the infinite one NaN
+    assert s[5, 0].isnan() and q.float()[5, :128].isnan().all() and (q.float()[5, 128:] == 0).all()
+
+
+# ---------------------------------------------------------------- SiLU * up
+# expf within 2 steps (4 u), of which e / (1 + e) reaches the sum; the sum, quotient and product: 7 u.
+# The scale adds its division; the quotient y / s has that error twice, 448 / amax and the product.
+SILU_S, SILU_D = 8 * U, 16 * U
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("packed", [False, True])
+@pytest.mark.parametrize("m,k", [(1, 64), (5, 128), (3, 192), (130, 576), (257, 2048), (1, 8192)])
+def test_silu_mul(m, k, packed, dtype):
+    x = _rand(m * 11 + k, m, 2 * k, dtype=dtype, spread=0.3)
+    q, s = _ops().silu_mul_fp8(x, packed=packed)
+    if packed:
+        g, u = (v.reshape(m, k).double() for v in x.view(m, k // 64, 2, 64).unbind(2))
+    else:
+        g, u = x[:, :k].double(), x[:, k:].double()
+    _check_quantized(q, s, g * torch.sigmoid(g) * u, d=SILU_D, s_tol=SILU_S)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_silu_mul_odd_widths_and_views(dtype):
+    wide = _rand(12, 40, 1000, dtype=dtype, spread=0.3)
+    for x in (wide[:, :2], wide[:, 1:255], wide[::2, 8:408], wide[:7, 3:997]):
+        q, s = _ops().silu_mul_fp8(x)
+        k = x.shape[1] // 2
+        g, u = x[:, :k].double(), x[:, k:].double()
+        _check_quantized(q, s, g * torch.sigmoid(g) * u, d=SILU_D, s_tol=SILU_S)
+    x = wide[::3, 5:5 + 256]
+    q, s = _ops().silu_mul_fp8(x, packed=True)
+    g, u = (v.reshape(x.shape[0], 128).double() for v in x.reshape(x.shape[0], 2, 2, 64).unbind(2))
+    _check_quantized(q, s, g * torch.sigmoid(g) * u, d=SILU_D, s_tol=SILU_S)
+
+
+@pytest.mark.gpu
+def test_silu_mul_far_gates():
+    """Gates whose exponential overflows or vanishes, and NaN."""
+    g = torch.tensor([-1e4, -200.0, -88.0, -50.0, 0.0, 50.0, 88.0, 200.0, 1e4], device=DEV)
+    x = torch.cat([g, torch.full_like(g, 2.0)])[None]
+    q, s = _ops().silu_mul_fp8(x)
+    _check_quantized(q, s, (g.double() * torch.sigmoid(g.double()) * 2)[None], d=SILU_D, s_tol=SILU_S)
+    x[0, 3] = float("nan")
+    q, s = _ops().silu_mul_fp8(x)
+    assert s.isnan().all() and q.float().isnan().all()
+
+
+# ---------------------------------------------------------------- linear
+LINEAR = [(1, 1, 1), (1, 16, 16), (1, 128, 128), (2, 130, 129), (5, 960, 576), (8, 256, 2048), (9, 6144, 2048),
+          (33, 2048, 8192), (64, 1000, 1000), (127, 300, 200), (128, 128, 640), (129, 257, 384), (320, 2048, 1024),
+          (513, 1024, 300), (1000, 1536, 576), (2049, 4100, 520), (3000, 5000, 130)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("out_f32", [False, True])
+@pytest.mark.parametrize("m,n,k", LINEAR)
+def test_linear(m, n, k, out_f32):
+    x, xs, w, ws = _operands(m + n + k, m, n, k)
+    y = _ops().linear_fp8(x, xs, w, ws, out_f32=out_f32)
+    _check_product(y, x, xs, w, ws, out_f32)
+
+
+@pytest.mark.gpu
+def test_linear_of_views():
+    """Rows off the 16-byte boundaries (copied), a column block of a wider matrix, strided scales."""
+    ops = _ops()
+    x, xs, w, ws = _operands(21, 40, 300, 512)
+    y = ops.linear_fp8(x, xs, w, ws, out_f32=True)
+    odd = torch.zeros(40, 515, dtype=torch.uint8, device=DEV).view(F8)
+    odd.view(torch.uint8)[:, 3:] = x.view(torch.uint8)
+    assert torch.equal(ops.linear_fp8(odd[:, 3:], xs, w, ws, out_f32=True), y)
+    wide = torch.zeros(300, 1024, dtype=torch.uint8, device=DEV).view(F8)
+    wide.view(torch.uint8)[:, 256:768] = w.view(torch.uint8)
+    assert torch.equal(ops.linear_fp8(x, xs, wide[:, 256:768], ws, out_f32=True), y)
+    assert torch.equal(ops.linear_fp8(x, xs.t().contiguous().t(), w, ws.t().contiguous().t(), out_f32=True), y)
+    one = ops.linear_fp8(odd[5:6, 3:], xs[5:6], w, ws, out_f32=True)
+    assert torch.equal(one, ops.linear_fp8(x[5:6].contiguous(), xs[5:6], w, ws, out_f32=True))
+
+
+@pytest.mark.gpu
+def test_linear_output_pitch_and_frame():
+    """Through the C ABI: an output with a pitch of its own (odd: scalar stores) keeps what lies around it."""
+    lib = _lib()
+    for m, n, k, pitch in ((5, 200, 256, 207), (130, 96, 128, 104), (40, 333, 2048, 340)):
+        x, xs, w, ws = _operands(m, m, n, k)
+        for f32 in (0, 1):
+            y = torch.full((m + 2, pitch), 9.0, dtype=F32 if f32 else BF16, device=DEV)
+            status = torch.full((1,), 77, dtype=torch.int32, device=DEV)
+            rc = lib.specb200_linear_fp8(x.data_ptr(), x.stride(0), xs.data_ptr(), w.data_ptr(), w.stride(0), ws.data_ptr(),
+                                         m, n, k, f32, y[1].data_ptr(), pitch, status.data_ptr(),
+                                         torch.cuda.current_stream().cuda_stream)
+            assert rc == 0 and int(status) == 0
+            assert (y[0] == 9).all() and (y[-1] == 9).all() and (y[:, n:] == 9).all()
+            _check_product(y[1:-1, :n], x, xs, w, ws, bool(f32))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", [(3, 300, 2048), (200, 384, 256)])
+def test_linear_keeps_nan_to_its_row(m, n, k):
+    """A NaN activation or scale reaches its own token, a NaN weight its own feature, and no others."""
+    ops = _ops()
+    x, xs, w, ws = _operands(31, m, n, k)
+    clean = ops.linear_fp8(x, xs, w, ws, out_f32=True)
+    x.view(torch.uint8)[1, 5] = 0x7F
+    w.view(torch.uint8)[17, 9] = 0xFF
+    xs[2, 1] = float("nan")
+    y = ops.linear_fp8(x, xs, w, ws, out_f32=True)
+    bad = torch.zeros_like(y, dtype=torch.bool)
+    bad[1] = bad[2] = True
+    bad[:, 17] = True
+    assert y[bad].isnan().all() and torch.equal(y[~bad], clean[~bad])
+
+
+@pytest.mark.gpu
+def test_linear_is_the_same_every_time_and_in_any_batch():
+    """Bit for bit: repeated, and with the other tokens of the call taken away where the plan is the same."""
+    ops = _ops()
+    x, xs, w, ws = _operands(41, 7, 2048, 8192)
+    y = ops.linear_fp8(x, xs, w, ws)
+    for _ in range(5):
+        assert torch.equal(ops.linear_fp8(x, xs, w, ws), y)
+    assert torch.equal(ops.linear_fp8(x[2:5], xs[2:5], w, ws), y[2:5])
+
+
+@pytest.mark.gpu
+def test_streams_and_graphs_do_not_share_state():
+    """Two streams that overlap, and two captured graphs replayed at once, give each call's own results."""
+    ops = _ops()
+    cases = [_operands(50 + i, m, n, k) for i, (m, n, k) in enumerate([(5, 2048, 8192), (40, 2048, 4096)])]
+    want = [ops.linear_fp8(*c) for c in cases]
+    acts = [_rand(60 + i, 50, 2048, dtype=BF16) for i in range(2)]
+    weight = torch.ones(2048, dtype=BF16, device=DEV)
+    norm = [ops.rmsnorm_fp8(a, weight, 1e-5, delta=a) for a in acts]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    got = [[] for _ in cases]
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append((ops.linear_fp8(*cases[i], check=False), ops.rmsnorm_fp8(acts[i], weight, 1e-5, delta=acts[i])))
+    torch.cuda.synchronize()
+    same = lambda a, b: all(torch.equal(p.view(torch.uint8), q.view(torch.uint8)) for p, q in zip(a, b))  # noqa: E731
+    for i in range(2):
+        for y, n in got[i]:
+            assert torch.equal(y, want[i]) and same(n, norm[i])
+    graphs = []
+    for i in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            y = ops.linear_fp8(*cases[i], check=False)
+            n = ops.rmsnorm_fp8(acts[i], weight, 1e-5, delta=acts[i])
+        graphs.append((g, y, n))
+    for _ in range(3):
+        for (g, _, _), s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for i, (_, y, n) in enumerate(graphs):
+        assert torch.equal(y, want[i]) and same(n, norm[i])
+
+
+# ---------------------------------------------------------------- together
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens", [1, 5, 160])
+def test_a_layer_of_8_bit_linears(tokens):
+    """A Llama layer's linears from 8-bit weights, with the engine's attention between them: every
+    step against its formula on the inputs it was given."""
+    ops = _ops()
+    hidden, heads, kv_heads, d, inter = 576, 9, 3, 64, 1024
+    qkv_n = (heads + 2 * kv_heads) * d
+    w = {name: ops.quantize_fp8((0.05 * _rand(i, *shape, spread=0.0)).to(BF16), block_rows=128)
+         for i, (name, shape) in enumerate([("qkv", (qkv_n, hidden)), ("o", (hidden, heads * d)),
+                                            ("gate_up", (2 * inter, hidden)), ("down", (hidden, inter))])}
+    ones = torch.ones(hidden, dtype=BF16, device=DEV)
+    x = _rand(70, tokens, hidden, dtype=BF16, spread=0.3)
+
+    def linear(q, s, name, out_f32=False):
+        y = ops.linear_fp8(q, s, *w[name], out_f32=out_f32)
+        _check_product(y, q, s, *w[name], out_f32)
+        return y
+
+    q, s = ops.rmsnorm_fp8(x, ones, 1e-5)
+    _check_quantized(q, s, _norm64(x, ones, 1e-5), d=4 * U, s_tol=NORM_S)
+    qkv = linear(q, s, "qkv")
+    block = 16
+    nblocks = -(-tokens // block)
+    k_pool = torch.zeros(nblocks * block, kv_heads, d, dtype=BF16, device=DEV)
+    v_pool = torch.zeros_like(k_pool)
+    parts = qkv.view(tokens, heads + 2 * kv_heads, d)
+    k_pool[:tokens], v_pool[:tokens] = parts[:, heads:heads + kv_heads], parts[:, heads + kv_heads:]
+    table = torch.arange(nblocks, dtype=torch.int32, device=DEV)[None]
+    zero, new = (torch.tensor([v], dtype=torch.int32, device=DEV) for v in (0, tokens))
+    att = ops.attention(parts[None, :, :heads].contiguous(), k_pool, v_pool, table, block, zero, new, d ** -0.5, tokens)
+    att = att.reshape(tokens, heads * d)
+    qa, sa = ops.quantize_fp8(att)
+    _check_quantized(qa, sa, att.double(), d=4 * U, s_tol=2 * U)
+    o = linear(qa, sa, "o")
+    q, s, h = ops.rmsnorm_fp8(x, ones, 1e-5, delta=o)
+    assert torch.equal(h, (x.float() + o.float()).to(BF16))
+    _check_quantized(q, s, _norm64(h, ones, 1e-5), d=4 * U, s_tol=NORM_S)
+    gu = linear(q, s, "gate_up")
+    q, s = ops.silu_mul_fp8(gu, packed=True)
+    g, u = (v.reshape(tokens, inter).double() for v in gu.view(tokens, inter // 64, 2, 64).unbind(2))
+    _check_quantized(q, s, g * torch.sigmoid(g) * u, d=SILU_D, s_tol=SILU_S)
+    down = linear(q, s, "down")
+    assert (h + down).isfinite().all()
