@@ -15,9 +15,13 @@ constexpr int kFp8Group = 128;
 constexpr float kE4m3Max = 448.f;
 constexpr float kFp8MinAmax = 7.888609052210118e-31f;  // 2^-100
 
-// Magnitudes are compared as the bit patterns of |x|: the order of the values, with every NaN
-// above infinity, so a NaN wins the maximum instead of being dropped by fmaxf.
-SPECB200_DEVINL uint32_t mag_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+// The larger magnitude, where a NaN wins: fmaxf would drop it, and a group's NaN has to reach its scale.
+SPECB200_DEVINL float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+SPECB200_DEVINL float max_mag(float m, float x) { return max_nan(m, fabsf(x)); }
 SPECB200_DEVINL float floor_amax(float amax) { return amax < kFp8MinAmax ? kFp8MinAmax : amax; }
 
 // Eight fp32 values as e4m3, rounded to nearest even; finite values beyond 448 (a group's

@@ -13,74 +13,125 @@
 namespace specb200 {
 namespace {
 
-// Eight consecutive elements of a row, `valid` of them inside it (the rest read as zero). vec:
-// the row starts on a 16-byte boundary.
+// Sixteen consecutive elements of a row, in the form they have in memory. align: every row starts
+// on a boundary of that many bytes: 32 takes 256-bit loads, 16 takes 128-bit ones, less one load
+// per element.
 template <typename T>
-SPECB200_DEVINL void load8(const T* p, int valid, bool vec, float (&f)[8]) {
-  if (vec && valid >= 8) {
-    if constexpr (sizeof(T) == 2) {
-      const uint4 v = __ldcg(reinterpret_cast<const uint4*>(p));
-      const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+struct Raw16 {
+  uint32_t v[4 * sizeof(T)];
+};
+template <typename T>
+SPECB200_DEVINL void load16(Raw16<T>& r, const T* p, int valid, int align) {
+  constexpr int kWords = 4 * sizeof(T);
+  if (align >= 16 && valid >= 16) {
+    const char* b = reinterpret_cast<const char*>(p);
+    if (align >= 32) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        f[2 * i] = __uint_as_float(u[i] << 16);
-        f[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
-      }
+      for (int i = 0; i < kWords; i += 8)
+        asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=r"(r.v[i]), "=r"(r.v[i + 1]), "=r"(r.v[i + 2]), "=r"(r.v[i + 3]), "=r"(r.v[i + 4]),
+                       "=r"(r.v[i + 5]), "=r"(r.v[i + 6]), "=r"(r.v[i + 7])
+                     : "l"(b + 4 * i));
     } else {
-      const float4 a = __ldcg(reinterpret_cast<const float4*>(p)), b = __ldcg(reinterpret_cast<const float4*>(p) + 1);
-      f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
-      f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+#pragma unroll
+      for (int i = 0; i < kWords; i += 4) {
+        const uint4 q = *reinterpret_cast<const uint4*>(b + 4 * i);
+        r.v[i] = q.x; r.v[i + 1] = q.y; r.v[i + 2] = q.z; r.v[i + 3] = q.w;
+      }
     }
     return;
   }
 #pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = i < valid ? to_f32<T>(p[i]) : 0.f;
-}
-
-template <typename T>
-SPECB200_DEVINL void store8(T* p, int valid, bool vec, const float (&f)[8]) {
-  if (vec && valid >= 8) {
-    if constexpr (sizeof(T) == 2) {
-      uint32_t u[4];
+  for (int i = 0; i < kWords; ++i) r.v[i] = 0;
+  if (valid <= 0) return;  // lanes behind a row's end: their warp need not go through the single loads
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < kWords; ++i) {
+    if constexpr (sizeof(T) == 2) {
+      const unsigned short* h = reinterpret_cast<const unsigned short*>(p);
+      const uint32_t lo = 2 * i < valid ? h[2 * i] : 0, hi = 2 * i + 1 < valid ? h[2 * i + 1] : 0;
+      r.v[i] = lo | (hi << 16);
+    } else {
+      r.v[i] = i < valid ? reinterpret_cast<const uint32_t*>(p)[i] : 0;
+    }
+  }
+}
+template <typename T>
+SPECB200_DEVINL void unpack16(const Raw16<T>& r, float (&f)[16]) {
+  if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      f[2 * i] = __uint_as_float(r.v[i] << 16);
+      f[2 * i + 1] = __uint_as_float(r.v[i] & 0xffff0000u);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(r.v[i]);
+  }
+}
+template <typename T>
+SPECB200_DEVINL void store16(T* p, int valid, int align, const float (&f)[16]) {
+  constexpr int kWords = 4 * sizeof(T);
+  if (align >= 16 && valid >= 16) {
+    uint32_t u[kWords];
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) {
+      if constexpr (sizeof(T) == 2) {
         const __nv_bfloat162 b = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
         u[i] = *reinterpret_cast<const uint32_t*>(&b);
+      } else {
+        u[i] = __float_as_uint(f[i]);
       }
-      *reinterpret_cast<uint4*>(p) = make_uint4(u[0], u[1], u[2], u[3]);
-    } else {
-      reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
-      reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
     }
+#pragma unroll
+    for (int i = 0; i < kWords; i += 4)
+      reinterpret_cast<uint4*>(p)[i / 4] = make_uint4(u[i], u[i + 1], u[i + 2], u[i + 3]);
     return;
   }
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
+  for (int i = 0; i < 16; ++i)
     if (i < valid) p[i] = from_f32<T>(f[i]);
 }
-
-SPECB200_DEVINL void store_q8(uint8_t* p, int valid, bool vec, const float (&f)[8]) {
-  const uint2 v = pack_e4m3(f);
-  if (vec && valid >= 8) {
-    *reinterpret_cast<uint2*>(p) = v;
+// e4m3(f * inv), 16 of a row.
+SPECB200_DEVINL void store_q16(uint8_t* p, int valid, int align, const float (&f)[16], float inv) {
+  uint32_t v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(f[4 * i] * inv, f[4 * i + 1] * inv), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(f[4 * i + 2] * inv, f[4 * i + 3] * inv), __NV_SATFINITE, __NV_E4M3);
+    v[i] = lo | (hi << 16);
+  }
+  if (align >= 16 && valid >= 16) {
+    *reinterpret_cast<uint4*>(p) = make_uint4(v[0], v[1], v[2], v[3]);
     return;
   }
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (i < valid) p[i] = static_cast<uint8_t>((i < 4 ? v.x : v.y) >> (8 * (i & 3)));
+  for (int i = 0; i < 16; ++i)
+    if (i < valid) p[i] = static_cast<uint8_t>(v[i / 4] >> (8 * (i & 3)));
 }
 
-SPECB200_DEVINL uint32_t max_mag8(const float (&f)[8]) {
-  uint32_t m = 0;
+SPECB200_DEVINL float max_mag16(const float (&f)[16]) {
+  float m = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) m = max(m, mag_bits(f[i]));
+  for (int i = 0; i < 16; ++i) m = max_mag(m, f[i]);
   return m;
 }
-// Maximum over the 16 lanes that hold a group.
-SPECB200_DEVINL uint32_t half_warp_max(uint32_t m) {
+// Maximum over the 8 lanes that hold a group.
+SPECB200_DEVINL float octet_max(float m) {
 #pragma unroll
-  for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+  for (int o = 4; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
   return m;
+}
+
+// silu(g) * u = g u / (1 + e^-g). The exponential is 2^t with t = -g log2(e), whose rounding is
+// carried along (2^(hi + lo) = 2^hi (1 + lo ln 2)): without it a far gate loses |g| 2^-24.
+SPECB200_DEVINL float silu_mul(float g, float u) {
+  constexpr float kLog2e = 1.44269504f, kLn2 = 0.69314718f;
+  const float hi = -g * kLog2e, lo = fmaf(-g, kLog2e, -hi);
+  float e, s;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(hi));
+  const float d = 1.f + (isfinite(hi) ? fmaf(e, lo * kLn2, e) : e);
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(d));
+  return g * s * u;
 }
 
 struct RowArgs {
@@ -91,80 +142,90 @@ struct RowArgs {
   float* scales;       // [M, groups] (or [row blocks, groups])
   int M, K, groups;
   int packed;          // SiLU: 1 = 64 gate columns, then their 64 up columns
-  int vec_in, vec_out; // rows of x / q start on 16- / 8-byte boundaries
+  int vec_in, vec_out; // rows of x / q start on boundaries of this many bytes
 };
 
 constexpr int kRowThreads = 256;
 
-// One group of one row per 16 lanes. kSilu: y = silu(gate) * up, else y = x.
+// One group of the row-major list of all groups per 8 lanes, 16 elements each. kSilu: y =
+// silu(gate) * up, else y = x. Bound by memory: what counts is loads in flight, so bf16 keeps to 32
+// registers (8 CTAs per SM); two groups per thread at 48 registers took longer at every size.
 template <typename T, bool kSilu>
-__global__ void __launch_bounds__(kRowThreads) quantize_rows_kernel(RowArgs a) {
+__global__ void __launch_bounds__(kRowThreads, sizeof(T) == 2 ? 8 : 5) quantize_rows_kernel(RowArgs a) {
   pdl_launch_dependents();
-  const int64_t unit = (static_cast<int64_t>(blockIdx.x) * kRowThreads + threadIdx.x) >> 4;
-  const int64_t units = static_cast<int64_t>(a.M) * a.groups;
-  pdl_wait();
-  const bool live = unit < units;
-  const int64_t row = live ? unit / a.groups : 0;
-  const int g = live ? static_cast<int>(unit - row * a.groups) : 0;
-  const int lane = threadIdx.x & 15;
-  const int col = g * kFp8Group + lane * 8;
-  const int valid = live ? min(8, max(0, a.K - col)) : 0;
+  const int lane = threadIdx.x & 7;
+  const uint32_t groups = a.groups;
+  const int64_t start = static_cast<int64_t>(blockIdx.x) * (kRowThreads / 8);  // the same in all threads
+  const int64_t row0 = start / groups;
+  const uint32_t at = static_cast<uint32_t>(start - row0 * groups) + (threadIdx.x >> 3);
+  const uint32_t over = at < groups ? 0u : at / groups;
+  const int64_t row = row0 + over;
+  const int g = static_cast<int>(at - over * groups), col = g * kFp8Group + lane * 16;
+  const int valid = row < a.M ? a.K - col : 0;
   const T* xr = static_cast<const T*>(a.x) + row * a.ldx;
-  float y[8];
+  pdl_wait();
+  Raw16<T> raw;
+  float y[16];
   if constexpr (kSilu) {
     // packed: feature j is gate column 128 (j / 64) + j % 64, its up column 64 further on
-    const int gate_col = a.packed ? ((col >> 6) << 7) + (col & 63) : col;
-    float u[8];
-    load8<T>(xr + gate_col, valid, a.vec_in, y);
-    load8<T>(xr + gate_col + (a.packed ? 64 : a.K), valid, a.vec_in, u);
+    const int gate = a.packed ? ((col >> 6) << 7) + (col & 63) : col;
+    Raw16<T> raw_up;
+    load16<T>(raw, xr + gate, valid, a.vec_in);
+    load16<T>(raw_up, xr + gate + (a.packed ? 64 : a.K), valid, a.vec_in);
+    float up[16];
+    unpack16<T>(raw, y);
+    unpack16<T>(raw_up, up);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = y[i] / (1.f + expf(-y[i])) * u[i];
+    for (int j = 0; j < 16; ++j) y[j] = silu_mul(y[j], up[j]);
   } else {
-    load8<T>(xr + col, valid, a.vec_in, y);
+    load16<T>(raw, xr + col, valid, a.vec_in);
+    unpack16<T>(raw, y);
   }
-  const float amax = floor_amax(__uint_as_float(half_warp_max(max_mag8(y))));
-  const float inv = kE4m3Max / amax;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) y[i] *= inv;
-  if (valid > 0) store_q8(a.q + row * a.ldq + col, valid, a.vec_out, y);
-  if (live && lane == 0) a.scales[unit] = amax / kE4m3Max;
+  const float amax = floor_amax(octet_max(max_mag16(y)));
+  if (valid > 0) store_q16(a.q + row * a.ldq + col, valid, a.vec_out, y, kE4m3Max / amax);
+  if (row < a.M && lane == 0) a.scales[row * groups + g] = amax / kE4m3Max;
 }
 
-// One 128 x 128 block per CTA, held in registers between the maximum and the rounding: 16 lanes
-// per row, 16 rows at a time.
+// One 128 x 128 block per CTA, held in registers between the maximum and the rounding: 8 lanes
+// per row, 32 rows at a time.
 template <typename T>
-__global__ void __launch_bounds__(kRowThreads) quantize_blocks_kernel(RowArgs a) {
-  constexpr int kPass = kFp8Group / (kRowThreads / 16);
-  __shared__ uint32_t sh[kRowThreads / 32];
+__global__ void __launch_bounds__(kRowThreads, sizeof(T) == 2 ? 3 : 2) quantize_blocks_kernel(RowArgs a) {
+  constexpr int kLanes = kRowThreads / 8, kPass = kFp8Group / kLanes;
+  __shared__ float sh[kRowThreads / 32];
   pdl_launch_dependents();
-  const int lane = threadIdx.x & 15, r0 = threadIdx.x >> 4;
+  const int lane = threadIdx.x & 7, r0 = threadIdx.x >> 3;
   const int g = blockIdx.x % a.groups, rb = blockIdx.x / a.groups;
-  const int col = g * kFp8Group + lane * 8;
-  const int valid = min(8, max(0, a.K - col));
+  const int col = g * kFp8Group + lane * 16;
+  const int valid = a.K - col;
+  const int rows = min(kFp8Group, a.M - rb * kFp8Group);
+  const int64_t first = static_cast<int64_t>(rb) * kFp8Group + r0;
+  const T* xp = static_cast<const T*>(a.x) + first * a.ldx + col;
+  uint8_t* qp = a.q + first * a.ldq + col;
   pdl_wait();
-  float y[kPass][8];
-  uint32_t m = 0;
+  Raw16<T> x[kPass];
+#pragma unroll
+  for (int p = 0; p < kPass; ++p)
+    load16<T>(x[p], xp + p * kLanes * a.ldx, r0 + p * kLanes < rows ? valid : 0, a.vec_in);
+  float m = 0.f;
 #pragma unroll
   for (int p = 0; p < kPass; ++p) {
-    const int row = rb * kFp8Group + p * (kRowThreads / 16) + r0;
-    const int64_t at = static_cast<int64_t>(min(row, a.M - 1)) * a.ldx + col;
-    load8<T>(static_cast<const T*>(a.x) + at, row < a.M ? valid : 0, a.vec_in, y[p]);
+    float y[16];
+    unpack16<T>(x[p], y);
+    m = max_nan(m, max_mag16(y));
   }
 #pragma unroll
-  for (int p = 0; p < kPass; ++p) m = max(m, max_mag8(y[p]));
-  m = __reduce_max_sync(0xffffffffu, m);
+  for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
   if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = m;
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < kRowThreads / 32; ++i) m = max(m, sh[i]);
-  const float amax = floor_amax(__uint_as_float(m));
+  for (int i = 0; i < kRowThreads / 32; ++i) m = max_nan(m, sh[i]);
+  const float amax = floor_amax(m);
   const float inv = kE4m3Max / amax;
 #pragma unroll
   for (int p = 0; p < kPass; ++p) {
-    const int row = rb * kFp8Group + p * (kRowThreads / 16) + r0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) y[p][i] *= inv;
-    if (row < a.M && valid > 0) store_q8(a.q + row * a.ldq + col, valid, a.vec_out, y[p]);
+    float y[16];
+    unpack16<T>(x[p], y);
+    if (r0 + p * kLanes < rows && valid > 0) store_q16(qp + p * kLanes * a.ldq, valid, a.vec_out, y, inv);
   }
   if (threadIdx.x == 0) a.scales[blockIdx.x] = amax / kE4m3Max;
 }
@@ -180,98 +241,151 @@ struct NormArgs {
   uint8_t* q;
   int64_t ldq;
   float* scales;
-  int H, groups;
+  int M, H, groups;
+  int rows;            // rows that a CTA takes at a time
   float eps;
-  int vec_x, vec_d, vec_w, vec_h, vec_q;
+  int vec_x, vec_d, vec_w, vec_h, vec_q;  // boundaries in bytes
 };
 
-constexpr int kNormMaxThreads = 1024;
-constexpr int kNormMaxChunks = 4;  // 8-element chunks per thread
-constexpr int kNormMaxWidth = kNormMaxThreads * kNormMaxChunks * 8;
+constexpr int kNormMaxChunks = 4;                            // groups of a row per 8 lanes
+constexpr int kNormMaxWidth = kNormMaxChunks * 64 * kFp8Group;  // 64 octets: 512 threads
 
-// h = T(x + delta); y = w h / sqrt(mean(h^2) + eps); (q, scales) = quantize(y). One CTA per row,
-// the row in registers.
+// CTAs per SM that the registers are cut for. 32768 x 2048 bf16 with delta, loads ahead: 72.9 us at 3
+// CTAs (98% of the measured bandwidth), 82.7 at 2, and 80.3 at 4 without room for loads ahead; fp32
+// 16384 x 2048: 68.7 at 2, 74.2 at 3. 8192 x 8192 bf16 (two groups per octet): 82.4 at 3, 88.8 at 2.
+template <typename T, int kChunks>
+constexpr int kNormCtas = kChunks == 4 ? 1 : kChunks == 2 ? 3 : sizeof(T) == 2 ? 3 : 2;
+
+// h = T(x + delta); y = w h / sqrt(mean(h^2) + eps); (q, scales) = quantize(y).
+//
+// Eight lanes hold one group of a row (kChunks groups of a wide one); a CTA takes as many rows at
+// a time as it has octets for, and walks over the rows with its weights in registers. With one group per
+// octet the next rows' loads are issued before the current rows' sums are formed. A row's sum of squares is added
+// within each octet by shuffles, then over the octets in a fixed order.
 //
 // The quantized values need no norm: with m the group's largest |w h| and r the row's 1 / rms,
 // y / s = (w h r) / (m r / 448) = w h (448 / m), so q carries two roundings and only the scale
 // waits for the row's sum. Where the floor is in play or a value is not finite, q is formed from
 // y itself.
-template <typename T, int kChunks>
-__global__ void __launch_bounds__(kNormMaxThreads) rmsnorm_fp8_kernel(NormArgs a) {
-  __shared__ float sh[kNormMaxThreads / 32];
+template <typename T, int kChunks, bool kDelta>
+__global__ void __launch_bounds__(kChunks == 4 ? 512 : 256, kNormCtas<T, kChunks>) rmsnorm_fp8_kernel(NormArgs a) {
+  constexpr bool kAhead = kChunks == 1;
+  __shared__ float sh[2][64];
   pdl_launch_dependents();
-  const int64_t row = blockIdx.x;
-  const int tid = threadIdx.x, nthr = blockDim.x;
-  pdl_wait();
-  const T* xr = static_cast<const T*>(a.x) + row * a.ldx;
-  float f[kChunks][8];
-#pragma unroll
-  for (int c = 0; c < kChunks; ++c) {
-    const int col = (tid + c * nthr) * 8;
-    load8<T>(xr + col, a.H - col, a.vec_x, f[c]);
-  }
-  if (a.delta) {
-    const T* dr = static_cast<const T*>(a.delta) + row * a.ldd;
-    T* hr = static_cast<T*>(a.h) + row * a.ldh;
+  const int octet = threadIdx.x >> 3, octets = blockDim.x >> 3;
+  const int per_row = min(octets, a.groups);  // octets that share a row
+  const int team = kChunks == 1 ? octet / per_row : 0;
+  const int g0 = octet - team * per_row;
+  const int col0 = g0 * kFp8Group + (threadIdx.x & 7) * 16;
+  const int pitch = octets * kFp8Group;  // from chunk to chunk of a thread
+  Raw16<T> w[kChunks], x[kChunks], d[kDelta ? kChunks : 1];
+  auto valid_of = [&](int64_t row, int c) { return team < a.rows && row < a.M ? a.H - (col0 + c * pitch) : 0; };
+  auto load_row = [&](int64_t row) {
 #pragma unroll
     for (int c = 0; c < kChunks; ++c) {
-      const int col = (tid + c * nthr) * 8;
-      float d[8];
-      load8<T>(dr + col, a.H - col, a.vec_d, d);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) f[c][i] = round_to<T>(f[c][i] + d[i]);
-      store8<T>(hr + col, a.H - col, a.vec_h, f[c]);
+      const int col = col0 + c * pitch, valid = valid_of(row, c);
+      load16<T>(x[c], static_cast<const T*>(a.x) + row * a.ldx + col, valid, a.vec_x);
+      if constexpr (kDelta) load16<T>(d[c], static_cast<const T*>(a.delta) + row * a.ldd + col, valid, a.vec_d);
     }
-  }
-  float ss = 0.f;
-  uint32_t m[kChunks];
+  };
+  const int64_t step = static_cast<int64_t>(gridDim.x) * a.rows;
+  int64_t base = static_cast<int64_t>(blockIdx.x) * a.rows;
+  pdl_wait();
+  if constexpr (kAhead) load_row(base + team);
 #pragma unroll
-  for (int c = 0; c < kChunks; ++c) {
-    const int col = (tid + c * nthr) * 8;
-    float w[8];
-    load8<T>(static_cast<const T*>(a.weight) + col, a.H - col, a.vec_w, w);
+  for (int c = 0; c < kChunks; ++c)
+    load16<T>(w[c], static_cast<const T*>(a.weight) + col0 + c * pitch, a.H - (col0 + c * pitch), a.vec_w);
+  for (int parity = 0; base < a.M; base += step, parity ^= 1) {
+    const int64_t row = base + team;
+    float f[kChunks][16], m[kChunks];
+    float ss = 0.f;
+    if constexpr (!kAhead) load_row(row);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      ss = fmaf(f[c][i], f[c][i], ss);
-      f[c][i] *= w[i];
+    for (int c = 0; c < kChunks; ++c) {
+      unpack16<T>(x[c], f[c]);
+      if constexpr (kDelta) {
+        float g[16];
+        unpack16<T>(d[c], g);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) f[c][i] = round_to<T>(f[c][i] + g[i]);
+      }
     }
-    m[c] = half_warp_max(max_mag8(f[c]));
-  }
-  ss = warp_sum(ss);
-  if ((tid & 31) == 0) sh[tid >> 5] = ss;
-  __syncthreads();
-  float total = 0.f;
-  for (int i = 0; i < nthr / 32; ++i) total += sh[i];
-  const float r = 1.f / sqrtf(total / static_cast<float>(a.H) + a.eps);
+    if constexpr (kAhead) {
+      if (base + step < a.M) load_row(row + step);
+    }
 #pragma unroll
-  for (int c = 0; c < kChunks; ++c) {
-    const int col = (tid + c * nthr) * 8;
-    const float top = __uint_as_float(m[c]);
-    const float amax = floor_amax(top * r);
-    // 2^-100 <= both and finite: 448 / top is finite and the row's factor cancels
-    const bool cancels = amax > kFp8MinAmax && amax <= 3.402823466e38f && top >= kFp8MinAmax;
-    const float inv = kE4m3Max / (cancels ? top : amax);
+    for (int c = 0; c < kChunks; ++c) {
+      const int col = col0 + c * pitch, valid = valid_of(row, c);
+      if constexpr (kDelta) {
+        if (valid > 0) store16<T>(static_cast<T*>(a.h) + row * a.ldh + col, valid, a.vec_h, f[c]);
+      }
+      float g[16], part = 0.f;
+      unpack16<T>(w[c], g);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[c][i] = (cancels ? f[c][i] : f[c][i] * r) * inv;
-    if (col < a.H) store_q8(a.q + row * a.ldq + col, a.H - col, a.vec_q, f[c]);
-    if (col < a.H && (tid & 15) == 0) a.scales[row * a.groups + col / kFp8Group] = amax / kE4m3Max;
+      for (int i = 0; i < 16; ++i) {
+        part = fmaf(f[c][i], f[c][i], part);
+        f[c][i] *= g[i];
+      }
+      ss += part;
+      m[c] = octet_max(max_mag16(f[c]));
+    }
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    if ((threadIdx.x & 7) == 0) sh[parity][octet] = ss;
+    __syncthreads();  // one per round: the next round's sums go to the other half
+    const float* part = &sh[parity][team * per_row];
+    float sums[4] = {0.f, 0.f, 0.f, 0.f};
+    if (team < a.rows) {
+      int i = 0;
+      for (; i + 4 <= per_row; i += 4) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sums[j] += part[i + j];
+      }
+      for (; i < per_row; ++i) sums[0] += part[i];
+    }
+    const float total = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+    const float r = 1.f / sqrtf(total / static_cast<float>(a.H) + a.eps);
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) {
+      const int col = col0 + c * pitch, valid = valid_of(row, c);
+      const float amax = floor_amax(m[c] * r);
+      // 2^-100 <= both and finite: 448 / m is finite and the row's factor cancels
+      const bool cancels = amax > kFp8MinAmax && amax <= 3.402823466e38f && m[c] >= kFp8MinAmax;
+      if (!cancels) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) f[c][i] *= r;
+      }
+      if (valid > 0) {
+        store_q16(a.q + row * a.ldq + col, valid, a.vec_q, f[c], kE4m3Max / (cancels ? m[c] : amax));
+        if ((threadIdx.x & 7) == 0) a.scales[row * a.groups + col / kFp8Group] = amax / kE4m3Max;
+      }
+    }
   }
 }
 
 int groups_of(int width) { return (width + kFp8Group - 1) / kFp8Group; }
 
+// The largest power of two up to 32 on whose multiples (in bytes) every row starts.
+int row_align(const void* p, int64_t pitch_bytes) {
+  int n = 32;
+  while (n > 1 && (reinterpret_cast<uintptr_t>(p) % n || pitch_bytes % n)) n /= 2;
+  return n;
+}
 template <typename T>
-bool rows_vec(const void* p, int64_t ld) {
-  return fp8_aligned(p, 16) && (ld * sizeof(T)) % 16 == 0;
+int row_align_of(const void* p, int64_t ld) {
+  return row_align(p, ld * static_cast<int64_t>(sizeof(T)));
+}
+
+unsigned row_ctas(const RowArgs& a) {
+  const int64_t units = static_cast<int64_t>(a.M) * a.groups, per_cta = kRowThreads / 8;
+  return static_cast<unsigned>((units + per_cta - 1) / per_cta);
 }
 
 template <typename T>
 cudaError_t launch_quantize(RowArgs a, int block_rows, cudaStream_t s) {
-  a.vec_in = rows_vec<T>(a.x, a.ldx);
+  a.vec_in = row_align_of<T>(a.x, a.ldx);
   if (block_rows == 1) {
-    const int64_t units = static_cast<int64_t>(a.M) * a.groups;
-    const int64_t ctas = (units * 16 + kRowThreads - 1) / kRowThreads;
-    return launch_kernel(quantize_rows_kernel<T, false>, dim3(static_cast<unsigned>(ctas)), dim3(kRowThreads), 0, s, true, a);
+    return launch_kernel(quantize_rows_kernel<T, false>, dim3(row_ctas(a)), dim3(kRowThreads), 0, s, true, a);
   }
   const unsigned blocks = static_cast<unsigned>(groups_of(a.M)) * a.groups;
   return launch_kernel(quantize_blocks_kernel<T>, dim3(blocks), dim3(kRowThreads), 0, s, true, a);
@@ -279,26 +393,38 @@ cudaError_t launch_quantize(RowArgs a, int block_rows, cudaStream_t s) {
 
 template <typename T>
 cudaError_t launch_silu_mul(RowArgs a, cudaStream_t s) {
-  a.vec_in = rows_vec<T>(a.x, a.ldx) && (a.packed || (static_cast<int64_t>(a.K) * sizeof(T)) % 16 == 0);
-  const int64_t units = static_cast<int64_t>(a.M) * a.groups;
-  const int64_t ctas = (units * 16 + kRowThreads - 1) / kRowThreads;
-  return launch_kernel(quantize_rows_kernel<T, true>, dim3(static_cast<unsigned>(ctas)), dim3(kRowThreads), 0, s, true, a);
+  a.vec_in = row_align_of<T>(a.x, a.ldx);
+  if (!a.packed) a.vec_in = std::min(a.vec_in, row_align_of<T>(a.x, a.K));  // where the up columns start
+  return launch_kernel(quantize_rows_kernel<T, true>, dim3(row_ctas(a)), dim3(kRowThreads), 0, s, true, a);
+}
+
+// As many CTAs as the 148 SMs hold at once, each on every grid-th set of rows.
+template <typename K>
+cudaError_t launch_filled(K kernel, const NormArgs& a, int threads, cudaStream_t s) {
+  int per_sm = 0;
+  const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, 0);
+  if (e != cudaSuccess) return e;
+  return launch_kernel(kernel, dim3(std::min((a.M - 1) / a.rows + 1, 148 * std::max(1, per_sm))), dim3(threads), 0, s, true, a);
+}
+template <typename T, int kChunks>
+cudaError_t launch_norm_kernel(const NormArgs& a, int octets, cudaStream_t s) {
+  const int threads = (octets * 8 + 31) / 32 * 32;
+  return a.delta ? launch_filled(rmsnorm_fp8_kernel<T, kChunks, true>, a, threads, s)
+                 : launch_filled(rmsnorm_fp8_kernel<T, kChunks, false>, a, threads, s);
 }
 
 template <typename T>
-cudaError_t launch_rmsnorm_fp8(NormArgs a, int M, cudaStream_t s) {
-  a.vec_x = rows_vec<T>(a.x, a.ldx);
-  a.vec_d = a.delta && rows_vec<T>(a.delta, a.ldd);
-  a.vec_w = fp8_aligned(a.weight, 16);
-  a.vec_h = a.delta && rows_vec<T>(a.h, a.ldh);
-  const int chunks = (a.H + 7) / 8;
-  // as many threads as chunks, up to 1024, in whole warps; then 2 or 4 chunks per thread
-  const int per = chunks <= kNormMaxThreads ? 1 : chunks <= 2 * kNormMaxThreads ? 2 : 4;
-  const int threads = ((chunks + per - 1) / per + 31) / 32 * 32;
-  const dim3 grid(static_cast<unsigned>(M)), block(threads);
-  if (per == 1) return launch_kernel(rmsnorm_fp8_kernel<T, 1>, grid, block, 0, s, true, a);
-  if (per == 2) return launch_kernel(rmsnorm_fp8_kernel<T, 2>, grid, block, 0, s, true, a);
-  return launch_kernel(rmsnorm_fp8_kernel<T, 4>, grid, block, 0, s, true, a);
+cudaError_t launch_rmsnorm_fp8(NormArgs a, cudaStream_t s) {
+  a.vec_x = row_align_of<T>(a.x, a.ldx);
+  a.vec_d = row_align_of<T>(a.delta, a.ldd);
+  a.vec_w = row_align(a.weight, 0);
+  a.vec_h = row_align_of<T>(a.h, a.ldh);
+  a.rows = 1;
+  if (a.groups > 64) return launch_norm_kernel<T, 4>(a, std::max(32, (a.groups + 3) / 4), s);
+  if (a.groups > 32) return launch_norm_kernel<T, 2>(a, (a.groups + 1) / 2, s);
+  // few rows: one per CTA, so that they spread over the SMs; many: as many as 32 octets hold
+  a.rows = std::max(1, std::min(32 / a.groups, a.M / (2 * 148)));
+  return launch_norm_kernel<T, 1>(a, a.rows * a.groups, s);
 }
 
 }  // namespace
@@ -334,7 +460,7 @@ extern "C" int specb200_quantize_fp8(int dtype, const void* x, int64_t ldx, int 
   a.M = M;
   a.K = K;
   a.groups = groups_of(K);
-  a.vec_out = fp8_aligned(q, 8) && ldq % 8 == 0;
+  a.vec_out = row_align(q, ldq);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return finish(dtype == SPECB200_BF16 ? launch_quantize<__nv_bfloat16>(a, block_rows, s) : launch_quantize<float>(a, block_rows, s));
 }
@@ -357,7 +483,7 @@ extern "C" int specb200_silu_mul_fp8(int dtype, const void* gate_up, int64_t ld,
   a.K = I;
   a.groups = groups_of(I);
   a.packed = packed ? 1 : 0;
-  a.vec_out = fp8_aligned(q, 8) && ldq % 8 == 0;
+  a.vec_out = row_align(q, ldq);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return finish(dtype == SPECB200_BF16 ? launch_silu_mul<__nv_bfloat16>(a, s) : launch_silu_mul<float>(a, s));
 }
@@ -382,10 +508,11 @@ extern "C" int specb200_rmsnorm_fp8(int dtype, const void* x, int64_t ldx, const
   a.q = static_cast<uint8_t*>(q);
   a.ldq = ldq;
   a.scales = scales;
+  a.M = M;
   a.H = H;
   a.groups = groups_of(H);
   a.eps = eps;
-  a.vec_q = fp8_aligned(q, 8) && ldq % 8 == 0;
+  a.vec_q = row_align(q, ldq);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return finish(dtype == SPECB200_BF16 ? launch_rmsnorm_fp8<__nv_bfloat16>(a, M, s) : launch_rmsnorm_fp8<float>(a, M, s));
+  return finish(dtype == SPECB200_BF16 ? launch_rmsnorm_fp8<__nv_bfloat16>(a, s) : launch_rmsnorm_fp8<float>(a, s));
 }

@@ -162,6 +162,12 @@ def stream_ptr(device: torch.device | None = None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def raw_stream(device: torch.device) -> int:
+    """stream_ptr without the Stream object in between (0.1 instead of 2.3 us of host time per call,
+    beside a launch of 4)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
 _HERE = contextlib.nullcontext()
 
 

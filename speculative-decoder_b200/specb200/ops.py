@@ -211,7 +211,7 @@ def quantize_fp8(x: torch.Tensor, block_rows: int = 1) -> tuple[torch.Tensor, to
     q, scales = _fp8_out(m, k, block_rows, dev)
     with _ffi.on_device(dev):
         rc = lib().specb200_quantize_fp8(code, ptr(rows), _pitch(rows), m, k, block_rows, ptr(q), q.stride(0),
-                                         ptr(scales), stream_ptr(dev))
+                                         ptr(scales), _ffi.raw_stream(dev))
     raise_for(rc, "specb200_quantize_fp8")
     return (q, scales) if x.dim() == 2 else _shaped(x.shape[:-1], q, scales)
 
@@ -238,7 +238,7 @@ def rmsnorm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float,
     with _ffi.on_device(dev):
         rc = lib().specb200_rmsnorm_fp8(code, ptr(rows), _pitch(rows), ptr(d), 0 if d is None else _pitch(d),
                                         ptr(weight), m, k, eps, ptr(h), k, ptr(q), q.stride(0), ptr(scales),
-                                        stream_ptr(dev))
+                                        _ffi.raw_stream(dev))
     raise_for(rc, "specb200_rmsnorm_fp8")
     out = (q, scales) if h is None else (q, scales, h)
     return out if x.dim() == 2 else _shaped(x.shape[:-1], *out)
@@ -256,7 +256,7 @@ def silu_mul_fp8(gate_up: torch.Tensor, packed: bool = False) -> tuple[torch.Ten
     q, scales = _fp8_out(m, both // 2, 1, dev)
     with _ffi.on_device(dev):
         rc = lib().specb200_silu_mul_fp8(code, ptr(rows), _pitch(rows), m, both // 2, int(packed), ptr(q),
-                                         q.stride(0), ptr(scales), stream_ptr(dev))
+                                         q.stride(0), ptr(scales), _ffi.raw_stream(dev))
     raise_for(rc, "specb200_silu_mul_fp8")
     return (q, scales) if gate_up.dim() == 2 else _shaped(gate_up.shape[:-1], q, scales)
 
@@ -297,7 +297,7 @@ def linear_fp8(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scale
     status = torch.empty(1, dtype=torch.int32, device=dev) if check else None
     with _ffi.on_device(dev):
         rc = lib().specb200_linear_fp8(ptr(rows), _pitch(rows), ptr(x_scales), ptr(w), _pitch(w), ptr(w_scales), m, n, k,
-                                       int(out_f32), ptr(y), n, ptr(status), stream_ptr(dev))
+                                       int(out_f32), ptr(y), n, ptr(status), _ffi.raw_stream(dev))
     raise_for(rc, "specb200_linear_fp8")
     if check:
         _ffi.check_status(status, "linear_fp8")

@@ -335,8 +335,9 @@ def test_nothing_is_written_outside_the_rows(op):
 
 
 # ---------------------------------------------------------------- RMSNorm
-# The sum of squares: at most 32 in a thread, 5 shuffles and 32 warps, so 69 roundings; half of
-# that in 1 / rms, then the mean, the sum with eps, the root, the quotient, w h, (w h) r and / 448.
+# The sum of squares: 16 in a chain, 4 chunks, 3 shuffles and 64 octets in 4 chains of 16 and their
+# join, so 41 roundings (69 allowed); half of that in 1 / rms, then the mean, the sum with eps, the
+# root, the quotient, w h, (w h) r and / 448.
 NORM_S = (69 / 2 + 7) * U
 
 
