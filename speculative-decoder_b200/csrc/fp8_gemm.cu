@@ -4,18 +4,18 @@
 //
 // The inner sum runs on the tensor cores (tcgen05.mma kind::f8f6f4, fp32 accumulator in TMEM);
 // its 128 products of one group share one pair of scales, so each group's partial tile is read
-// back and added to fp32 registers with the factor sx * sw. Two TMEM buffers alternate: the MMA
-// of group b + 1 runs while group b is added.
+// back and added to fp32 registers with the factor sx * sw, while the MMAs of the next group run
+// into another TMEM buffer. Tokens lie on the TMEM lanes: a thread owns one token and features of
+// one weight block, so the factor of a group is one number per thread. Operands come by TMA, K-major
+// with the 128-byte swizzle (one atom is one group). Two kernels:
 //
-// A CTA computes a tile of 128 tokens x BN features, tokens on the TMEM lanes: a thread then
-// owns one token and 64 features of one weight block, and the factor of a group is one number per
-// thread. Warp roles: kEpi epilogue warps (warp w reads TMEM lane quarter w % 4, columns
-// 64 (w / 4)..), then a warp that issues TMA (both operands K-major with the 128-byte swizzle: one
-// atom is one group) and a warp that issues tcgen05.mma.
-//
-// With few tiles K is split over the CTAs of a cluster. Each leaves its partial tile in its own
-// shared memory and the cluster adds them through distributed shared memory in split order, so
-// results do not depend on scheduling and no workspace exists that two calls could share.
+// - gemm_fp8_small_kernel: a CTA computes one tile of 128 tokens x 128 features, two CTAs per SM.
+//   With few tiles K is split over the CTAs of a cluster: each leaves its partial tile in its own
+//   shared memory and the cluster adds them through distributed shared memory in split order, so
+//   results do not depend on scheduling and no workspace exists that two calls could share.
+// - gemm_fp8_pair_kernel: a pair of CTAs (cta_group::2) walks over tiles of 256 tokens x 256
+//   features. Each CTA loads half of either operand, so that a group costs an SM 32 KB from L2
+//   instead of 48, and holds 128 tokens of the accumulators.
 #include <algorithm>
 #include <atomic>
 
@@ -26,22 +26,16 @@ namespace specb200 {
 namespace {
 
 constexpr int kF8TileM = 128;
-constexpr int kF8Cols = 64;  // features per epilogue thread
+constexpr int kF8Block = 128;     // features per weight block
 constexpr int kF8MaxSplits = 8;
 constexpr int kF8MaxStages = 12;
 constexpr int kF8MaxDevices = 64;
-constexpr int kF8OutBytes = 2048;  // per epilogue warp: 32 rows x 64 bytes of output on their way to memory
-
-// Epilogue warps of a BN-wide tile, and the block around them (with a whole fifth warpgroup
-// where registers are redistributed).
-__host__ __device__ constexpr int f8_epi_warps(int bn) { return bn / kF8Cols * 4; }
-__host__ __device__ constexpr int f8_threads(int bn) { return bn == 256 ? 640 : 320; }
-
-struct F8Barriers {
-  uint64_t full[kF8MaxStages], empty[kF8MaxStages], tfull[2], tempty[2];
-  uint32_t tmem_holder;
-  int abort_flag;
-};
+constexpr int kF8EpiWarps = 8;
+constexpr int kF8SmallThreads = 320;
+constexpr int kF8PairThreads = 384;
+constexpr int kF8PairStages = 4;
+constexpr int kF8OutPiece = 4096; // 32 rows x 128 bytes of output on their way to memory
+constexpr uint32_t kF8TileBytes = 128 * kFp8Group;  // 128 rows of one group
 
 struct F8Args {
   int M, N, K;
@@ -52,29 +46,44 @@ struct F8Args {
   const float* ws;      // [n / 128, kblocks]
   void* y;
   int64_t ldy;
-  int out_f32, vec_y;
+  int out_f32;
+  int rows16;           // y's rows are on 16-byte boundaries: tiles are written by TMA, split ones in quads
   int32_t* status;
 };
 
-// The MMAs of one group (128 of K in four instructions), overwriting the accumulator, and the two
-// commits: the stage is free and the accumulator complete once they have run. Every lane of the
-// warp executes this, the elected one (leader != 0) issues.
+// The MMAs of one group (128 of K in four instructions), overwriting the accumulator, and a commit:
+// `done` completes once they have run, here and (kPair) in the peer CTA. Every lane of the warp
+// executes this, the elected one (leader != 0) issues.
+template <bool kPair>
 SPECB200_DEVINL void umma_group_e4m3(uint32_t leader, uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc,
-                                     uint64_t* stage_free, uint64_t* acc_full) {
-  asm volatile(
-      "{\n\t.reg .pred p, first, rest;\n\t"
-      "setp.ne.b32 p, %0, 0;\n\t"
-      "setp.ne.b32 first, 0, 0;\n\t"
-      "setp.eq.b32 rest, 0, 0;\n\t"
-      "@p tcgen05.mma.cta_group::1.kind::f8f6f4 [%1], %2, %6, %10, first;\n\t"
-      "@p tcgen05.mma.cta_group::1.kind::f8f6f4 [%1], %3, %7, %10, rest;\n\t"
-      "@p tcgen05.mma.cta_group::1.kind::f8f6f4 [%1], %4, %8, %10, rest;\n\t"
-      "@p tcgen05.mma.cta_group::1.kind::f8f6f4 [%1], %5, %9, %10, rest;\n\t"
-      "@p tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%11];\n\t"
-      "@p tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%12];\n\t}" ::"r"(leader),
-      "r"(tmem_d), "l"(a), "l"(a + 2), "l"(a + 4), "l"(a + 6), "l"(b), "l"(b + 2), "l"(b + 4), "l"(b + 6), "r"(idesc),
-      "r"(smem_u32(stage_free)), "r"(smem_u32(acc_full))
-      : "memory");
+                                     uint64_t* done) {
+  if constexpr (kPair) {
+    asm volatile(
+        "{\n\t.reg .pred p, first, rest;\n\t"
+        "setp.ne.b32 p, %0, 0;\n\t"
+        "setp.ne.b32 first, 0, 0;\n\t"
+        "setp.eq.b32 rest, 0, 0;\n\t"
+        "@p tcgen05.mma.cta_group::2.kind::f8f6f4 [%1], %2, %6, %10, first;\n\t"
+        "@p tcgen05.mma.cta_group::2.kind::f8f6f4 [%1], %3, %7, %10, rest;\n\t"
+        "@p tcgen05.mma.cta_group::2.kind::f8f6f4 [%1], %4, %8, %10, rest;\n\t"
+        "@p tcgen05.mma.cta_group::2.kind::f8f6f4 [%1], %5, %9, %10, rest;\n\t"
+        "@p tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%11], %12;\n\t}" ::"r"(leader), "r"(tmem_d), "l"(a), "l"(a + 2),
+        "l"(a + 4), "l"(a + 6), "l"(b), "l"(b + 2), "l"(b + 4), "l"(b + 6), "r"(idesc), "r"(smem_u32(done)), "h"(static_cast<unsigned short>(3))
+        : "memory");
+  } else {
+    asm volatile(
+        "{\n\t.reg .pred p, first, rest;\n\t"
+        "setp.ne.b32 p, %0, 0;\n\t"
+        "setp.ne.b32 first, 0, 0;\n\t"
+        "setp.eq.b32 rest, 0, 0;\n\t"
+        "@p tcgen05.mma.cta_group::1.kind::f8f6f4 [%1], %2, %6, %10, first;\n\t"
+        "@p tcgen05.mma.cta_group::1.kind::f8f6f4 [%1], %3, %7, %10, rest;\n\t"
+        "@p tcgen05.mma.cta_group::1.kind::f8f6f4 [%1], %4, %8, %10, rest;\n\t"
+        "@p tcgen05.mma.cta_group::1.kind::f8f6f4 [%1], %5, %9, %10, rest;\n\t"
+        "@p tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%11];\n\t}" ::"r"(leader), "r"(tmem_d), "l"(a), "l"(a + 2),
+        "l"(a + 4), "l"(a + 6), "l"(b), "l"(b + 2), "l"(b + 4), "l"(b + 6), "r"(idesc), "r"(smem_u32(done))
+        : "memory");
+  }
 }
 SPECB200_DEVINL uint32_t elect_leader() {
   uint32_t r;
@@ -82,13 +91,19 @@ SPECB200_DEVINL uint32_t elect_leader() {
   return r;
 }
 
-// Bounded wait of a whole warp: every lane polls (no broadcast on the fast path) and all take the
-// same way out. Gives up as mbar_wait_bounded does.
-SPECB200_DEVINL bool wait_warp(uint64_t* bar, uint32_t parity, int32_t* status, volatile int* abort) {
-  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+// Bounded wait of a whole warp for a phase of one barrier, or of two: every lane polls (no broadcast
+// on the fast path) and all take the same way out. Gives up as mbar_wait_bounded does.
+template <bool kTwo>
+SPECB200_DEVINL bool wait_warp(uint64_t* bar, uint32_t parity, uint64_t* bar2, uint32_t parity2, int32_t* status,
+                               volatile int* abort) {
+  auto ready = [&] {
+    const bool a = mbar_try_wait(bar, parity), b = !kTwo || mbar_try_wait(bar2, parity2);
+    return __all_sync(0xffffffffu, a && b) != 0;
+  };
+  if (ready()) return true;
   const long long start = clock64();
   while (true) {
-    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    if (ready()) return true;
     const bool late = clock64() - start > SPECB200_SPIN_LIMIT_CYCLES;
     if (late) {
       set_status(status, SPECB200_ERR_TIMEOUT);
@@ -96,6 +111,9 @@ SPECB200_DEVINL bool wait_warp(uint64_t* bar, uint32_t parity, int32_t* status, 
     }
     if (__any_sync(0xffffffffu, late || *abort)) return false;
   }
+}
+SPECB200_DEVINL bool wait_warp(uint64_t* bar, uint32_t parity, int32_t* status, volatile int* abort) {
+  return wait_warp<false>(bar, parity, nullptr, 0, status, abort);
 }
 
 // Instruction descriptor, kind::f8f6f4: fp32 accumulator (bits 4-5 = 1), e4m3 A and B (bits 7-9
@@ -128,13 +146,60 @@ SPECB200_DEVINL void tmem_ld<16>(uint32_t taddr, uint32_t (&r)[16]) {
       : "r"(taddr));
 }
 
+template <>
+SPECB200_DEVINL void tmem_ld<8>(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr));
+}
+
 SPECB200_DEVINL void cluster_arrive_wait() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-SPECB200_DEVINL float4 ld_cluster_f4(uint32_t addr, uint32_t rank) {
+SPECB200_DEVINL uint32_t cluster_addr(uint32_t addr, uint32_t rank) {
   uint32_t r;
-  float4 v;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+SPECB200_DEVINL uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+SPECB200_DEVINL void mbar_arrive_cluster_if(bool cond, uint32_t addr) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %1, 0;\n\t@p mbarrier.arrive.shared::cluster.b64 _, [%0];\n\t}" ::"r"(addr),
+      "r"(static_cast<int>(cond))
+      : "memory");
+}
+// A load into this CTA's memory that completes on a barrier of the CTA pair's first CTA.
+SPECB200_DEVINL void tma_load_2d_pair(void* smem_dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, "
+      "%4}], [%2];" ::"r"(smem_u32(smem_dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1)
+      : "memory");
+}
+template <bool kPair>
+SPECB200_DEVINL void f8_tmem_alloc(uint32_t* holder, uint32_t cols) {
+  if constexpr (kPair) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(holder)), "r"(cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  } else {
+    tmem_alloc(holder, cols);
+    tmem_relinquish();
+  }
+}
+template <bool kPair>
+SPECB200_DEVINL void f8_tmem_dealloc(uint32_t taddr, uint32_t cols) {
+  if constexpr (kPair)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols) : "memory");
+  else
+    tmem_dealloc(taddr, cols);
+}
+SPECB200_DEVINL float4 ld_cluster_f4(uint32_t addr, uint32_t rank) {
+  const uint32_t r = cluster_addr(addr, rank);
+  float4 v;
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
                : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
                : "r"(r)
@@ -146,7 +211,7 @@ SPECB200_DEVINL float4 ld_cluster_f4(uint32_t addr, uint32_t rank) {
 SPECB200_DEVINL void store_quad(const F8Args& a, int64_t at, int valid, const float (&v)[4]) {
   if (a.out_f32) {
     float* p = static_cast<float*>(a.y) + at;
-    if (a.vec_y && valid >= 4) {
+    if (a.rows16 && valid >= 4) {
       *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
       return;
     }
@@ -156,7 +221,7 @@ SPECB200_DEVINL void store_quad(const F8Args& a, int64_t at, int valid, const fl
     return;
   }
   __nv_bfloat16* p = static_cast<__nv_bfloat16*>(a.y) + at;
-  if (a.vec_y && valid >= 4) {
+  if (a.rows16 && valid >= 4) {
     const __nv_bfloat162 b0 = __floats2bfloat162_rn(v[0], v[1]), b1 = __floats2bfloat162_rn(v[2], v[3]);
     *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&b0), *reinterpret_cast<const uint32_t*>(&b1));
     return;
@@ -166,85 +231,122 @@ SPECB200_DEVINL void store_quad(const F8Args& a, int64_t at, int valid, const fl
     if (i < valid) p[i] = __float2bfloat16_rn(v[i]);
 }
 
-// One warp's 32 tokens x 64 features to memory through 2 KB of shared memory, so that rows are
-// written in 64-byte pieces: 32 bf16 or 16 fp32 features at a time. The 16-byte units of a row are
-// swizzled by the row so that neither side has bank conflicts.
-template <typename T>
-SPECB200_DEVINL void store_warp_tile(const F8Args& a, const float (&acc)[kF8Cols], uint8_t* buf, int m0, int n0, int lane) {
-  constexpr int kUnit = 16 / sizeof(T), kPiece = 4 * kUnit;
-  const int row = lane >> 2, unit = lane & 3;
+// A scale, loaded here and not where the compiler would rather have it: a group ahead of its use.
+SPECB200_DEVINL float load_scale(const float* p) {
+  float v;
+  asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(v) : "l"(p));
+  return v;
+}
+
+// Four bytes to shared memory, and an arrival at `bar` once this thread's copies so far are there.
+SPECB200_DEVINL void copy_async_4(float* dst, const float* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+SPECB200_DEVINL void copy_async_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+SPECB200_DEVINL void tma_store_2d(const CUtensorMap* map, const void* smem_src, int c0, int c1) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(smem_u32(smem_src)), "r"(c0), "r"(c1)
+               : "memory");
+}
+
+// One warp's 32 tokens x kCols features to memory through kPieces pieces of shared memory, a piece
+// being 128 bytes per row (64 bf16 or 32 fp32 features). The 16-byte units of a row are swizzled by
+// the row (the 128-byte swizzle TMA reads), so that neither side has bank conflicts. TMA stores
+// leave the warp free while the pieces drain; an output whose rows are off the 16-byte boundaries is
+// written by the warp itself.
+template <typename T, int kPieces, int kCols>
+SPECB200_DEVINL void store_warp_tile(const F8Args& a, const CUtensorMap& y_map, const float (&acc)[kCols],
+                                     uint8_t* bufs, int m0, int n0, int lane) {
+  constexpr int kUnit = 16 / sizeof(T), kPiece = 8 * kUnit;
+  constexpr int kRound = kPieces * kPiece < kCols ? kPieces * kPiece : kCols;
 #pragma unroll
-  for (int c = 0; c < kF8Cols; c += kPiece) {
+  for (int c0 = 0; c0 < kCols; c0 += kRound) {
+    if (a.rows16) {  // what lay in the buffers has been read
+      if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+      __syncwarp();
+    }
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int c = c0; c < c0 + kRound; c += kUnit) {
       uint32_t v[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         if constexpr (sizeof(T) == 2) {
-          const __nv_bfloat162 b = __floats2bfloat162_rn(acc[c + u * kUnit + 2 * j], acc[c + u * kUnit + 2 * j + 1]);
+          const __nv_bfloat162 b = __floats2bfloat162_rn(acc[c + 2 * j], acc[c + 2 * j + 1]);
           v[j] = *reinterpret_cast<const uint32_t*>(&b);
         } else {
-          v[j] = __float_as_uint(acc[c + u * kUnit + j]);
+          v[j] = __float_as_uint(acc[c + j]);
         }
       }
-      *reinterpret_cast<uint4*>(buf + lane * 64 + (u ^ ((lane >> 1) & 3)) * 16) = make_uint4(v[0], v[1], v[2], v[3]);
+      const int piece = (c - c0) / kPiece, unit = (c - c0) % kPiece / kUnit;
+      *reinterpret_cast<uint4*>(bufs + piece * kF8OutPiece + lane * 128 + ((unit ^ lane) & 7) * 16) =
+          make_uint4(v[0], v[1], v[2], v[3]);
+    }
+    if (a.rows16) {
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) {
+#pragma unroll
+        for (int c = c0; c < c0 + kRound; c += kPiece)
+          if (n0 + c < a.N) tma_store_2d(&y_map, bufs + (c - c0) / kPiece * kF8OutPiece, n0 + c, m0);
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+      }
+      continue;
     }
     __syncwarp();
-    const int n = n0 + c + unit * kUnit, left = a.N - n;
+    for (int c = c0; c < c0 + kRound; c += kPiece) {
+      const int n = n0 + c + (lane & 7) * kUnit;
+      for (int r = lane >> 3; r < 32; r += 4) {
+        const uint4 q = *reinterpret_cast<const uint4*>(bufs + (c - c0) / kPiece * kF8OutPiece + r * 128 + ((lane ^ r) & 7) * 16);
+        const T* e = reinterpret_cast<const T*>(&q);
+        T* y = static_cast<T*>(a.y) + static_cast<int64_t>(m0 + r) * a.ldy + n;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = row + 8 * i, m = m0 + r;
-      const uint4 q = *reinterpret_cast<const uint4*>(buf + r * 64 + (unit ^ ((r >> 1) & 3)) * 16);
-      if (m < a.M && left > 0) {
-        T* p = static_cast<T*>(a.y) + static_cast<int64_t>(m) * a.ldy + n;
-        if (a.vec_y && left >= kUnit) {
-          *reinterpret_cast<uint4*>(p) = q;
-        } else {
-          const T* e = reinterpret_cast<const T*>(&q);
-#pragma unroll
-          for (int j = 0; j < kUnit; ++j)
-            if (j < left) p[j] = e[j];
-        }
+        for (int j = 0; j < kUnit; ++j)
+          if (m0 + r < a.M && n + j < a.N) y[j] = e[j];
       }
     }
     __syncwarp();
   }
 }
 
-template <int BN>
-__global__ void __launch_bounds__(f8_threads(BN), BN == 128 ? 2 : 1)
-    gemm_fp8_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map, F8Args a) {
-  constexpr int kEpi = f8_epi_warps(BN), kThreads = f8_threads(BN);
-  constexpr int kLd = BN == 256 ? 32 : 16;  // accumulator columns read back at a time (what registers allow)
-  constexpr int kPitch = BN + 4;            // partial tile's row pitch (floats)
-  constexpr uint32_t kWBytes = BN * kFp8Group;
-  // output staging, the ring (1024-byte swizzle atoms), then the barriers
+// ------------------------------------------------------------------------------ small tiles
+struct F8SmallBarriers {
+  uint64_t full[kF8MaxStages], done[kF8MaxStages], tempty[2];
+  uint32_t tmem_holder;
+  int abort_flag;
+};
+
+// Warps 0-7 read back (w on TMEM lane quarter w % 4, columns 64 (w / 4)..), warp 8 issues TMA, warp 9
+// tcgen05.mma. A stage's `done` barrier frees its operands and completes its accumulator.
+__global__ void __launch_bounds__(kF8SmallThreads, 2)
+    gemm_fp8_small_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map,
+                          const __grid_constant__ CUtensorMap y_map, F8Args a) {
+  constexpr int kCols = 64;                  // features per epilogue thread
+  constexpr int kLd = 16;                    // accumulator columns read back at a time (what registers allow)
+  constexpr int kPitch = kF8Block + 4;       // partial tile's row pitch (floats)
+  // the ring (1024-byte swizzle atoms), which ends up holding the output; then the barriers
   extern __shared__ __align__(1024) uint8_t smem[];
-  uint8_t* ring = smem + kEpi * kF8OutBytes;
-  F8Barriers& bars = *reinterpret_cast<F8Barriers*>(ring + a.ring_bytes);
-  uint64_t *full = bars.full, *empty = bars.empty, *tfull = bars.tfull, *tempty = bars.tempty;
+  F8SmallBarriers& bars = *reinterpret_cast<F8SmallBarriers*>(smem + a.ring_bytes);
+  uint64_t *full = bars.full, *done = bars.done, *tempty = bars.tempty;
   uint32_t& tmem_holder = bars.tmem_holder;
   int& abort_flag = bars.abort_flag;
-  const uint32_t stage_bytes = kWBytes + a.x_bytes;
+  const uint32_t stage_bytes = kF8TileBytes + a.x_bytes;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t stages = a.stages;
 
   if (threadIdx.x == 0) {
     for (uint32_t i = 0; i < stages; ++i) {
       mbar_init(&full[i], 1);
-      mbar_init(&empty[i], 1);
+      mbar_init(&done[i], 1);
     }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&tfull[i], 1);
-      mbar_init(&tempty[i], kEpi);
-    }
+    for (int i = 0; i < 2; ++i) mbar_init(&tempty[i], kF8EpiWarps);
     abort_flag = 0;
     fence_mbar_init();
   }
-  if (warp == kEpi + 1) {
-    tmem_alloc(&tmem_holder, 2 * BN);
-    tmem_relinquish();
-  }
+  if (warp == 9) f8_tmem_alloc<false>(&tmem_holder, 2 * kF8Block);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -253,135 +355,122 @@ __global__ void __launch_bounds__(f8_threads(BN), BN == 128 ? 2 : 1)
   // waited for it would keep it from ever starting.
   pdl_launch_dependents();
 
-  const int splits = a.splits;
-  const int split = splits > 1 ? static_cast<int>(blockIdx.x) % splits : 0;
-  const int first = static_cast<int>(blockIdx.x) / splits, step = static_cast<int>(gridDim.x) / splits;
-  const int tiles = a.m_tiles * a.n_tiles;
+  // a cluster is one tile, its CTAs the splits of K
+  const int splits = a.splits, split = static_cast<int>(blockIdx.x) % splits, tile = static_cast<int>(blockIdx.x) / splits;
+  const int tile_m = tile % a.m_tiles * kF8TileM, tile_n = tile / a.m_tiles * kF8Block;
   const int kb0 = static_cast<int>(static_cast<int64_t>(a.kblocks) * split / splits);
   const int kb1 = static_cast<int>(static_cast<int64_t>(a.kblocks) * (split + 1) / splits);
 
-  // 640 threads start with 96 registers each, 61,440; the shares below sum to 57,344 + 4,096.
-  if (warp >= kEpi) {
-    if constexpr (BN == 256) asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
-    if (warp == kEpi && lane == 0) {
+  if (warp == 8) {
+    if (lane == 0) {
       tma_prefetch_desc(&w_map);
       tma_prefetch_desc(&x_map);
       pdl_wait();
       uint32_t st = 0, phase = 0, issued = 0;
       bool ok = true;
-      for (int t = first; t < tiles && ok; t += step) {
-        const int m0 = (t % a.m_tiles) * kF8TileM, n0 = (t / a.m_tiles) * BN;
-        for (int kb = kb0; kb < kb1; ++kb) {
-          if (!mbar_wait_bounded(&empty[st], phase ^ 1, a.status, &abort_flag)) { ok = false; break; }
-          uint8_t* s = ring + st * stage_bytes;
-          mbar_arrive_expect_tx(&full[st], stage_bytes);
-          tma_load_2d(s, &w_map, &full[st], kb * kFp8Group, n0);
-          tma_load_2d(s + kWBytes, &x_map, &full[st], kb * kFp8Group, m0);
-          if (issued < stages) ++issued;
-          if (++st == stages) { st = 0; phase ^= 1; }
-        }
+      for (int kb = kb0; kb < kb1; ++kb) {
+        ok = mbar_wait_bounded(&done[st], phase ^ 1, a.status, &abort_flag);
+        if (!ok) break;
+        uint8_t* s = smem + st * stage_bytes;
+        mbar_arrive_expect_tx(&full[st], stage_bytes);
+        tma_load_2d(s, &w_map, &full[st], kb * kFp8Group, tile_n);
+        tma_load_2d(s + kF8TileBytes, &x_map, &full[st], kb * kFp8Group, tile_m);
+        if (issued < stages) ++issued;
+        if (++st == stages) { st = 0; phase ^= 1; }
       }
-      // Tail: the last use of every stage is released (so no commit arrives after the exit), or,
-      // where a wait gave up, at least every copy in flight has landed.
+      // Tail: the last use of every stage is done (so no commit arrives after the exit), or, where
+      // a wait gave up, at least every copy in flight has landed.
       for (uint32_t i = 0; i < issued; ++i) {
         if (st == 0) { st = stages; phase ^= 1; }
         --st;
-        if (ok) ok = mbar_wait_bounded(&empty[st], phase, a.status, &abort_flag);
+        if (ok) ok = mbar_wait_bounded(&done[st], phase, a.status, &abort_flag);
         if (!ok) mbar_wait_bounded(&full[st], phase, a.status, nullptr);
       }
-    } else if (warp == kEpi + 1) {
-      constexpr uint32_t idesc = umma_idesc_e4m3(kF8TileM, BN);
-      const uint32_t leader = elect_leader();
-      const uint64_t dw0 = umma_desc_sw128(smem_u32(ring)), dx0 = umma_desc_sw128(smem_u32(ring + kWBytes));
-      uint32_t st = 0, phase = 0, buf = 0, acc_phase = 0;
-      bool ok = true;
-      for (int t = first; t < tiles && ok; t += step) {
-        for (int kb = kb0; kb < kb1; ++kb) {
-          ok = wait_warp(&tempty[buf], acc_phase ^ 1, a.status, &abort_flag) &&
-               wait_warp(&full[st], phase, a.status, &abort_flag);
-          if (!ok) break;
-          tc_fence_after();
-          const uint64_t at = static_cast<uint64_t>(st * (stage_bytes >> 4));
-          umma_group_e4m3(leader, tmem + buf * BN, dx0 + at, dw0 + at, idesc, &empty[st], &tfull[buf]);
-          if (++st == stages) { st = 0; phase ^= 1; }
-          buf ^= 1;
-          acc_phase ^= buf ^ 1;
-        }
-      }
     }
-    __syncwarp();
+  } else if (warp == 9) {
+    constexpr uint32_t idesc = umma_idesc_e4m3(kF8TileM, kF8Block);
+    const uint32_t leader = elect_leader();
+    const uint64_t dw0 = umma_desc_sw128(smem_u32(smem)), dx0 = umma_desc_sw128(smem_u32(smem + kF8TileBytes));
+    uint32_t st = 0, phase = 0, buf = 0, acc_phase = 0;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (!wait_warp(&tempty[buf], acc_phase ^ 1, a.status, &abort_flag) ||
+          !wait_warp(&full[st], phase, a.status, &abort_flag))
+        break;
+      tc_fence_after();
+      const uint64_t at = static_cast<uint64_t>(st * (stage_bytes >> 4));
+      umma_group_e4m3<false>(leader, tmem + buf * kF8Block, dx0 + at, dw0 + at, idesc, &done[st]);
+      if (++st == stages) { st = 0; phase ^= 1; }
+      buf ^= 1;
+      acc_phase ^= buf ^ 1;
+    }
   } else {
-    if constexpr (BN == 256) asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
     pdl_wait();
-    const int quarter = warp & 3, col0 = (warp >> 2) * kF8Cols;
+    const int quarter = warp & 3, col0 = (warp >> 2) * kCols;
     const uint32_t tbase = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + col0;
-    uint32_t buf = 0, acc_phase = 0;
+    const int m0 = tile_m + quarter * 32, n0 = tile_n + col0;
+    const bool live = m0 < a.M && n0 < a.N;  // warps without outputs only keep step
+    const float* sx = a.xs + static_cast<int64_t>(min(m0 + lane, a.M - 1)) * a.kblocks;
+    const float* sw = a.ws + static_cast<int64_t>(tile_n / kF8Block) * a.kblocks;
+    float acc[kCols];
+#pragma unroll
+    for (int i = 0; i < kCols; ++i) acc[i] = 0.f;
+    float fx = live ? load_scale(sx + kb0) : 0.f, fw = live ? load_scale(sw + kb0) : 0.f;
+    uint32_t st = 0, phase = 0, buf = 0;
     bool ok = true;
-    for (int t = first; t < tiles && ok; t += step) {
-      const int m0 = (t % a.m_tiles) * kF8TileM + quarter * 32, n0 = (t / a.m_tiles) * BN + col0;
-      const bool live = m0 < a.M && n0 < a.N;  // warps without outputs only keep step
-      const float* sx = a.xs + static_cast<int64_t>(min(m0 + lane, a.M - 1)) * a.kblocks;
-      const float* sw = a.ws + static_cast<int64_t>(min(n0, a.N - 1) / kFp8Group) * a.kblocks;
-      float acc[kF8Cols];
-#pragma unroll
-      for (int i = 0; i < kF8Cols; ++i) acc[i] = 0.f;
-      float fx = live ? __ldg(sx + kb0) : 0.f, fw = live ? __ldg(sw + kb0) : 0.f;
-      for (int kb = kb0; kb < kb1; ++kb) {
-        const float f = fx * fw;
-        if (live && kb + 1 < kb1) {
-          fx = __ldg(sx + kb + 1);
-          fw = __ldg(sw + kb + 1);
-        }
-        ok = wait_warp(&tfull[buf], acc_phase, a.status, &abort_flag);
-        if (!ok) break;
-        tc_fence_after();
-        if (live) {
-#pragma unroll
-          for (int c = 0; c < kF8Cols; c += kLd) {
-            uint32_t r[kLd];
-            tmem_ld<kLd>(tbase + buf * BN + c, r);
-            tmem_ld_wait();
-            if (c + kLd == kF8Cols) {  // all read: the next but one group may overwrite it
-              tc_fence_before();
-              if (lane == 0) mbar_arrive(&tempty[buf]);
-            }
-#pragma unroll
-            for (int i = 0; i < kLd; ++i) acc[c + i] = fmaf(__uint_as_float(r[i]), f, acc[c + i]);
-          }
-        } else if (lane == 0) {
-          mbar_arrive(&tempty[buf]);
-        }
-        buf ^= 1;
-        acc_phase ^= buf ^ 1;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      const float f = fx * fw;
+      if (live && kb + 1 < kb1) {
+        fx = load_scale(sx + kb + 1);
+        fw = load_scale(sw + kb + 1);
       }
+      ok = wait_warp(&done[st], phase, a.status, &abort_flag);
       if (!ok) break;
-      if (splits == 1) {
-        if (live) {
-          if (a.out_f32)
-            store_warp_tile<float>(a, acc, smem + warp * kF8OutBytes, m0, n0, lane);
-          else
-            store_warp_tile<__nv_bfloat16>(a, acc, smem + warp * kF8OutBytes, m0, n0, lane);
+      tc_fence_after();
+      if (live) {
+#pragma unroll
+        for (int c = 0; c < kCols; c += kLd) {
+          uint32_t r[kLd];
+          tmem_ld<kLd>(tbase + buf * kF8Block + c, r);
+          tmem_ld_wait();
+          if (c + kLd == kCols) {  // all read: the next but one group may overwrite it
+            tc_fence_before();
+            if (lane == 0) mbar_arrive(&tempty[buf]);
+          }
+#pragma unroll
+          for (int i = 0; i < kLd; ++i) acc[c + i] = fmaf(__uint_as_float(r[i]), f, acc[c + i]);
         }
-      } else if (live) {  // one tile per cluster: every stage has been read, the ring holds the partial tile
-        float* p = reinterpret_cast<float*>(ring) + (quarter * 32 + lane) * kPitch + col0;
+      } else if (lane == 0) {
+        mbar_arrive(&tempty[buf]);
+      }
+      if (++st == stages) { st = 0; phase ^= 1; }
+      buf ^= 1;
+    }
+    // every group is done: the ring is idle and takes the output, or this split's partial tile
+    if (ok && live) {
+      if (splits > 1) {
+        float* p = reinterpret_cast<float*>(smem) + (quarter * 32 + lane) * kPitch + col0;
         if (m0 + lane < a.M) {
 #pragma unroll
-          for (int i = 0; i < kF8Cols; i += 4) *reinterpret_cast<float4*>(p + i) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
+          for (int i = 0; i < kCols; i += 4) *reinterpret_cast<float4*>(p + i) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
         }
+      } else if (a.out_f32) {
+        store_warp_tile<float, 1>(a, y_map, acc, smem + warp * kF8OutPiece, m0, n0, lane);
+      } else {
+        store_warp_tile<__nv_bfloat16, 1>(a, y_map, acc, smem + warp * kF8OutPiece, m0, n0, lane);
       }
     }
+    if (a.rows16 && splits == 1 && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
   __syncwarp();
   if (splits > 1) {
     cluster_arrive_wait();
-    const int m0 = (first % a.m_tiles) * kF8TileM, n0 = (first / a.m_tiles) * BN;
-    const int rows = min(kF8TileM, a.M - m0);
-    constexpr int kQuads = BN / 4;
+    const int rows = min(kF8TileM, a.M - tile_m);
+    constexpr int kQuads = kF8Block / 4;
     if (!*reinterpret_cast<volatile int*>(&abort_flag)) {
-      const uint32_t base = smem_u32(ring);
-      for (int i = split * kThreads + threadIdx.x; i < rows * kQuads; i += splits * kThreads) {
+      const uint32_t base = smem_u32(smem);
+      for (int i = split * kF8SmallThreads + threadIdx.x; i < rows * kQuads; i += splits * kF8SmallThreads) {
         const int r = i / kQuads, c = (i % kQuads) * 4;
-        if (n0 + c >= a.N) continue;
+        if (tile_n + c >= a.N) continue;
         float v[4] = {0.f, 0.f, 0.f, 0.f};
         for (int p0 = 0; p0 < splits; p0 += 4) {  // four splits' loads in flight, added in split order
           float4 q[4];
@@ -392,83 +481,353 @@ __global__ void __launch_bounds__(f8_threads(BN), BN == 128 ? 2 : 1)
           for (int j = 0; j < 4; ++j)
             if (p0 + j < splits) { v[0] += q[j].x; v[1] += q[j].y; v[2] += q[j].z; v[3] += q[j].w; }
         }
-        store_quad(a, static_cast<int64_t>(m0 + r) * a.ldy + n0 + c, a.N - n0 - c, v);
+        store_quad(a, static_cast<int64_t>(tile_m + r) * a.ldy + tile_n + c, a.N - tile_n - c, v);
       }
     }
     cluster_arrive_wait();  // no CTA leaves while another reads its shared memory
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == kEpi + 1) {
+  if (warp == 9) {
     tc_fence_after();
-    tmem_dealloc(tmem, 2 * BN);
+    f8_tmem_dealloc<false>(tmem, 2 * kF8Block);
+  }
+}
+
+// ------------------------------------------------------------------------------ CTA pairs
+// The scales of one group: of the CTA's 128 tokens and of the tile's two weight blocks.
+struct F8Scales {
+  float x[kF8TileM], w[4];
+};
+constexpr int kF8Slots = kF8PairStages + 2;
+struct F8PairBarriers {
+  uint64_t full[kF8PairStages], done[2][kF8PairStages], sfull[kF8Slots], tempty[2][2];
+  uint32_t tmem_holder;
+  int abort_flag;
+  F8Scales scales[kF8Slots];
+};
+constexpr int kF8PairPieces = 2;  // per epilogue warp: its whole bf16 tile
+constexpr size_t kF8PairOut = static_cast<size_t>(kF8EpiWarps) * kF8PairPieces * kF8OutPiece;
+constexpr size_t kF8PairSmem = kF8PairOut + kF8PairStages * 2 * kF8TileBytes + sizeof(F8PairBarriers);
+static_assert(kF8PairSmem <= 227 * 1024, "shared memory of a CTA");
+
+// A group's 256 features are multiplied in two halves with a TMEM buffer each (two groups' worth in
+// all): half h holds features 64 h..64 h + 63 of either weight block, so that each epilogue thread reads 64
+// columns of a half. What a buffer costs besides its MMAs -- the commit's and the release's way
+// between warps and CTAs, the read -- then hides behind three other buffers' MMAs; with one buffer per group it
+// did not (8192 x 16384 x 2048: 253 us).
+// Warps 0-7 read back (w on TMEM lane quarter w % 4, weight block w / 4), warp 8 issues TMA, warps 9
+// and 10 of the pair's first CTA tcgen05.mma for both (MMAs issue in order and block the warp while the
+// tensor cores are busy, so two warps take turns), warp 11 fetches scales.
+__global__ void __launch_bounds__(kF8PairThreads, 1)
+    gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map,
+                         const __grid_constant__ CUtensorMap y_map, F8Args a) {
+  constexpr int kCols = 128, kLd = 32;  // features per epilogue thread; columns read back at a time
+  constexpr uint32_t kStageBytes = 2 * kF8TileBytes;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint8_t* ring = smem + kF8PairOut;
+  F8PairBarriers& bars = *reinterpret_cast<F8PairBarriers*>(ring + kF8PairStages * kStageBytes);
+  int& abort_flag = bars.abort_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kF8PairStages; ++i) {
+      mbar_init(&bars.full[i], 1);
+      mbar_init(&bars.done[0][i], 1);
+      mbar_init(&bars.done[1][i], 1);
+    }
+    for (int i = 0; i < kF8Slots; ++i) mbar_init(&bars.sfull[i], 32);
+    for (int i = 0; i < 4; ++i) mbar_init(&bars.tempty[i >> 1][i & 1], 2 * kF8EpiWarps);
+    abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 9) f8_tmem_alloc<true>(&bars.tmem_holder, 512);
+  tc_fence_before();
+  __syncwarp();
+  cluster_arrive_wait();  // the peer's barriers are ready, too
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bars.tmem_holder;
+  pdl_launch_dependents();  // as in the small kernel, after the allocation
+
+  const int rank = static_cast<int>(cluster_rank());
+  const int first = static_cast<int>(blockIdx.x) / 2, step = static_cast<int>(gridDim.x) / 2;
+  const int tiles = a.m_tiles * a.n_tiles, kblocks = a.kblocks;
+  auto tile_m = [&](int t) { return (t % a.m_tiles * 2 + rank) * kF8TileM; };
+  auto tile_n = [&](int t) { return t / a.m_tiles * 2 * kF8Block; };
+
+  // 384 threads start with 168 registers each, 64,512; the shares below sum to 7,168 + 57,344.
+  if (warp >= kF8EpiWarps) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == 8) {
+      if (lane == 0) {
+        tma_prefetch_desc(&w_map);
+        tma_prefetch_desc(&x_map);
+        pdl_wait();
+        uint32_t st = 0, phase = 0, issued = 0;
+        bool ok = true;
+        for (int t = first; t < tiles && ok; t += step) {
+          const int m0 = tile_m(t), n0 = tile_n(t) + rank * kF8Block;
+          for (int kb = 0; kb < kblocks; ++kb) {
+            ok = mbar_wait_bounded(&bars.done[1][st], phase ^ 1, a.status, &abort_flag);
+            if (!ok) break;
+            uint8_t* s = ring + st * kStageBytes;
+            if (rank == 0) mbar_arrive_expect_tx(&bars.full[st], 2 * kStageBytes);  // both CTAs' loads
+            const uint32_t bar = cluster_addr(smem_u32(&bars.full[st]), 0);
+            tma_load_2d_pair(s, &w_map, bar, kb * kFp8Group, n0);
+            tma_load_2d_pair(s + kF8TileBytes, &x_map, bar, kb * kFp8Group, m0);
+            if (issued < kF8PairStages) ++issued;
+            if (++st == kF8PairStages) { st = 0; phase ^= 1; }
+          }
+        }
+        // Tail: the last use of every stage is done (so no commit arrives after the exit), or, where
+        // a wait gave up, at least every copy in flight has had its time to land.
+        for (uint32_t i = 0; i < issued; ++i) {
+          if (st == 0) { st = kF8PairStages; phase ^= 1; }
+          --st;
+          if (ok) ok = mbar_wait_bounded(&bars.done[1][st], phase, a.status, &abort_flag);
+          if (!ok) mbar_wait_bounded(rank == 0 ? &bars.full[st] : &bars.done[1][st], phase, a.status, nullptr);
+        }
+      }
+    } else if (warp == 11) {
+      // The scales, into a ring of two slots more than there are stages: once the stage of group g
+      // is done, the epilogue has read the scales of group g - 2 (the MMAs of g waited for that),
+      // whose slot and barrier come next.
+      pdl_wait();
+      uint32_t st = 0, phase = 0, slot = 0;
+      bool ok = true;
+      for (int t = first; t < tiles && ok; t += step) {
+        const int m0 = tile_m(t) + lane, block = tile_n(t) / kF8Block + lane;
+        const float* sx = a.xs + static_cast<int64_t>(m0) * kblocks;
+        const float* sw = a.ws + static_cast<int64_t>(block) * kblocks;
+        const int64_t pitch = static_cast<int64_t>(32) * kblocks;
+        const bool live_w = lane < 2 && block * kF8Block < a.N;
+        for (int kb = 0; kb < kblocks; ++kb) {
+          ok = wait_warp(&bars.done[1][st], phase ^ 1, a.status, &abort_flag);
+          if (!ok) break;
+          F8Scales& to = bars.scales[slot];
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (m0 + 32 * i < a.M) copy_async_4(&to.x[32 * i + lane], sx + i * pitch + kb);
+          if (live_w) copy_async_4(&to.w[lane], sw + kb);
+          copy_async_arrive(&bars.sfull[slot]);
+          if (++st == kF8PairStages) { st = 0; phase ^= 1; }
+          if (++slot == kF8Slots) slot = 0;
+        }
+      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
+    } else if (rank == 0) {  // warps 9 and 10: every other group each
+      constexpr uint32_t idesc = umma_idesc_e4m3(2 * kF8TileM, kF8Block);
+      const uint32_t leader = elect_leader();
+      const uint64_t dw0 = umma_desc_sw128(smem_u32(ring)), dx0 = umma_desc_sw128(smem_u32(ring + kF8TileBytes));
+      const uint32_t turn = static_cast<uint32_t>(warp - 9);
+      uint32_t st = 0, phase = 0, buf = 0, acc_phase = 0;
+      bool ok = true;
+      for (int t = first; t < tiles && ok; t += step) {
+        for (int kb = 0; kb < kblocks; ++kb) {
+          if (buf == turn) {
+            const uint64_t at = static_cast<uint64_t>(st * (kStageBytes >> 4));
+            ok = wait_warp<true>(&bars.tempty[buf][0], acc_phase ^ 1, &bars.full[st], phase, a.status, &abort_flag);
+            if (!ok) break;
+            tc_fence_after();
+            umma_group_e4m3<true>(leader, tmem + buf * 256, dx0 + at, dw0 + at, idesc, &bars.done[0][st]);
+            ok = wait_warp(&bars.tempty[buf][1], acc_phase ^ 1, a.status, &abort_flag);
+            if (!ok) break;
+            tc_fence_after();
+            umma_group_e4m3<true>(leader, tmem + buf * 256 + kF8Block, dx0 + at, dw0 + at + (kF8TileBytes >> 5), idesc,
+                                  &bars.done[1][st]);
+          }
+          if (++st == kF8PairStages) { st = 0; phase ^= 1; }
+          buf ^= 1;
+          acc_phase ^= buf ^ 1;
+        }
+      }
+    }
+    __syncwarp();
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    pdl_wait();
+    const int quarter = warp & 3, block = warp >> 2;
+    const uint32_t tbase = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + block * 64;
+    const uint32_t tempty0 = cluster_addr(smem_u32(bars.tempty), 0);  // the issuing CTA's
+    uint8_t* out_buf = smem + warp * (kF8PairPieces * kF8OutPiece);
+    uint32_t buf = 0, st = 0, phase = 0, slot = 0, slot_phase = 0;
+    bool ok = true;
+    // this half is read: the next but one group may overwrite it
+    auto release = [&](int half) {
+      tc_fence_before();
+      mbar_arrive_cluster_if(lane == 0, tempty0 + (buf * 2 + half) * sizeof(uint64_t));
+    };
+    auto next_group = [&] {
+      buf ^= 1;
+      if (++st == kF8PairStages) { st = 0; phase ^= 1; }
+      if (++slot == kF8Slots) { slot = 0; slot_phase ^= 1; }
+    };
+    // A poll (`try_`) is issued early, its outcome looked at (`ready`) where it is needed.
+    auto try_first = [&] { return mbar_try_wait(&bars.done[0][st], phase) && mbar_try_wait(&bars.sfull[slot], slot_phase); };
+    auto first_ready = [&](bool tried) {
+      return __all_sync(0xffffffffu, tried) ||
+             wait_warp<true>(&bars.done[0][st], phase, &bars.sfull[slot], slot_phase, a.status, &abort_flag);
+    };
+    auto try_second = [&] { return mbar_try_wait(&bars.done[1][st], phase); };
+    auto second_ready = [&](bool tried) {
+      return __all_sync(0xffffffffu, tried) || wait_warp(&bars.done[1][st], phase, a.status, &abort_flag);
+    };
+    auto factor = [&] { return bars.scales[slot].x[quarter * 32 + lane] * bars.scales[slot].w[block]; };
+    for (int t = first; t < tiles && ok; t += step) {
+      const int m0 = tile_m(t) + quarter * 32, n0 = tile_n(t) + block * kF8Block;
+      if (m0 >= a.M || n0 >= a.N) {  // a warp without outputs only keeps step
+        for (int kb = 0; kb < kblocks; ++kb) {
+          ok = first_ready(false) && second_ready(false);
+          if (!ok) break;
+          release(0);
+          release(1);
+          next_group();
+        }
+        continue;
+      }
+      float acc[kCols];
+#pragma unroll
+      for (int i = 0; i < kCols; ++i) acc[i] = 0.f;
+      // 32 columns come back at a time, the next ones and the next poll on their way while the last
+      // ones are added.
+      uint32_t r0[kLd], r1[kLd];
+      auto add = [&](int c, const uint32_t (&r)[kLd], float f) {
+#pragma unroll
+        for (int i = 0; i < kLd; ++i) acc[c + i] = fmaf(__uint_as_float(r[i]), f, acc[c + i]);
+      };
+      ok = first_ready(try_first());
+      if (!ok) break;
+      tc_fence_after();
+      float f = factor();
+      tmem_ld<kLd>(tbase + buf * 256, r0);
+      for (int kb = 0;;) {
+        const uint32_t at = tbase + buf * 256;
+        tmem_ld_wait();
+        tmem_ld<kLd>(at + 32, r1);
+        const bool second = try_second();
+        add(0, r0, f);
+        tmem_ld_wait();
+        release(0);
+        ok = second_ready(second);
+        if (!ok) break;
+        tc_fence_after();
+        tmem_ld<kLd>(at + 128, r0);
+        add(32, r1, f);
+        tmem_ld_wait();
+        tmem_ld<kLd>(at + 160, r1);
+        const uint32_t last = buf;
+        next_group();
+        const bool more = ++kb < kblocks, next = more && try_first();
+        add(64, r0, f);
+        tmem_ld_wait();
+        tc_fence_before();
+        mbar_arrive_cluster_if(lane == 0, tempty0 + (last * 2 + 1) * sizeof(uint64_t));
+        if (!more) {
+          add(96, r1, f);
+          break;
+        }
+        ok = first_ready(next);
+        if (!ok) break;
+        tc_fence_after();
+        tmem_ld<kLd>(tbase + buf * 256, r0);
+        const float f1 = factor();
+        add(96, r1, f);
+        f = f1;
+      }
+      if (!ok) break;
+      if (a.out_f32)
+        store_warp_tile<float, kF8PairPieces>(a, y_map, acc, out_buf, m0, n0, lane);
+      else
+        store_warp_tile<__nv_bfloat16, kF8PairPieces>(a, y_map, acc, out_buf, m0, n0, lane);
+    }
+    if (a.rows16 && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    __syncwarp();
+  }
+  tc_fence_before();
+  cluster_arrive_wait();  // every arrival at the other's barriers has landed
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    f8_tmem_dealloc<true>(tmem, 512);
   }
 }
 
 // ------------------------------------------------------------------------------ host side
 struct F8Plan {
-  int bn, splits, stages, box_rows;
+  bool pair;
+  int splits, stages, box_rows;
   int kblocks, m_tiles, n_tiles;
   size_t ring, smem;
 };
 
 F8Plan plan_fp8(int M, int N, int K) {
-  F8Plan p;
+  F8Plan p = {};
   p.kblocks = (K + kFp8Group - 1) / kFp8Group;
-  p.m_tiles = (M + kF8TileM - 1) / kF8TileM;
-  const int wide = (N + 255) / 256;
-  p.bn = static_cast<int64_t>(p.m_tiles) * wide >= 2 * 148 ? 256 : 128;
-  p.n_tiles = (N + p.bn - 1) / p.bn;
+  const int pair_m = (M + 2 * kF8TileM - 1) / (2 * kF8TileM), pair_n = (N + 2 * kF8Block - 1) / (2 * kF8Block);
+  p.pair = M > kF8TileM && static_cast<int64_t>(pair_m) * pair_n >= 148;
   p.splits = 1;
-  const int64_t tiles = static_cast<int64_t>(p.m_tiles) * p.n_tiles;
-  if (p.bn == 128)
-    while (p.splits < kF8MaxSplits && tiles * p.splits * 2 <= 2 * 148 && p.kblocks >= 4 * p.splits) p.splits *= 2;
   p.box_rows = std::min(kF8TileM, (M + 7) / 8 * 8);
-  const size_t x_bytes = static_cast<size_t>(p.box_rows) * kFp8Group, stage = p.bn * kFp8Group + x_bytes;
+  if (p.pair) {
+    p.m_tiles = pair_m;
+    p.n_tiles = pair_n;
+    p.stages = kF8PairStages;
+    p.smem = kF8PairSmem;
+    return p;
+  }
+  p.m_tiles = (M + kF8TileM - 1) / kF8TileM;
+  p.n_tiles = (N + kF8Block - 1) / kF8Block;
+  const int64_t tiles = static_cast<int64_t>(p.m_tiles) * p.n_tiles;
+  while (p.splits < kF8MaxSplits && tiles * p.splits * 2 <= 2 * 148 && p.kblocks >= 4 * p.splits) p.splits *= 2;
+  const size_t x_bytes = static_cast<size_t>(p.box_rows) * kFp8Group, stage = kF8TileBytes + x_bytes;
   // An MMA reads 128 token rows: with fewer in a box it runs on into the next stage, whose lanes
   // are never read back; the last stage needs that much room behind it.
-  const size_t slack = kF8TileM * kFp8Group - x_bytes;
+  const size_t slack = kF8TileBytes - x_bytes;
   // 228 KB per SM, of which each CTA takes 1 KB for itself: 113 KB each for two CTAs
-  const size_t fixed = static_cast<size_t>(f8_epi_warps(p.bn)) * kF8OutBytes + sizeof(F8Barriers);
-  const size_t budget = (p.bn == 128 ? 113 * 1024 : 227 * 1024) - fixed;
+  const size_t budget = 113 * 1024 - sizeof(F8SmallBarriers);
   p.stages = static_cast<int>(std::min<size_t>(kF8MaxStages, (budget - slack) / stage));
-  p.ring = p.stages * stage + slack;
-  if (p.splits > 1) p.ring = std::max(p.ring, static_cast<size_t>(p.box_rows) * (p.bn + 4) * 4);
-  p.smem = fixed + p.ring;
+  p.ring = std::max(p.stages * stage + slack, p.splits > 1 ? static_cast<size_t>(p.box_rows) * (kF8Block + 4) * 4
+                                                           : static_cast<size_t>(kF8EpiWarps) * kF8OutPiece);
+  p.smem = p.ring + sizeof(F8SmallBarriers);
   return p;
 }
 
-template <int BN>
-cudaError_t launch_fp8(const F8Plan& p, const CUtensorMap& wm, const CUtensorMap& xm, const F8Args& a, cudaStream_t s) {
-  // the attribute belongs to the current device's copy of the kernel
-  static std::atomic<bool> ready[kF8MaxDevices];
+// The attributes belong to the current device's copy of the kernel.
+template <typename K>
+cudaError_t prepare_fp8(K kernel, std::atomic<bool> (&ready)[kF8MaxDevices]) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || (dev < kF8MaxDevices && ready[dev].load(std::memory_order_acquire))) return e;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+  if (e == cudaSuccess && dev < kF8MaxDevices) ready[dev].store(true, std::memory_order_release);
+  return e;
+}
+
+cudaError_t launch_fp8(const F8Plan& p, const CUtensorMap& wm, const CUtensorMap& xm, const CUtensorMap& ym, const F8Args& a,
+                       cudaStream_t s) {
+  static std::atomic<bool> small_ready[kF8MaxDevices], pair_ready[kF8MaxDevices];
+  const cudaError_t e = p.pair ? prepare_fp8(gemm_fp8_pair_kernel, pair_ready) : prepare_fp8(gemm_fp8_small_kernel, small_ready);
   if (e != cudaSuccess) return e;
-  if (dev >= kF8MaxDevices || !ready[dev].load(std::memory_order_acquire)) {
-    e = cudaFuncSetAttribute(gemm_fp8_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
-    if (e != cudaSuccess) return e;
-    e = cudaFuncSetAttribute(gemm_fp8_kernel<BN>, cudaFuncAttributePreferredSharedMemoryCarveout,
-                             cudaSharedmemCarveoutMaxShared);
-    if (e != cudaSuccess) return e;
-    if (dev < kF8MaxDevices) ready[dev].store(true, std::memory_order_release);
-  }
   const int64_t tiles = static_cast<int64_t>(p.m_tiles) * p.n_tiles;
+  const int cluster = p.pair ? 2 : p.splits;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(p.splits > 1 ? tiles * p.splits : std::min<int64_t>(tiles, BN == 128 ? 296 : 148)));
-  cfg.blockDim = dim3(f8_threads(BN));
+  cfg.gridDim = dim3(static_cast<unsigned>((p.pair ? std::min<int64_t>(tiles, 74) : tiles) * cluster));
+  cfg.blockDim = dim3(p.pair ? kF8PairThreads : kF8SmallThreads);
   cfg.dynamicSmemBytes = p.smem;
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = p.splits;
+  attr[1].val.clusterDim.x = cluster;
   attr[1].val.clusterDim.y = 1;
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = p.splits > 1 ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, gemm_fp8_kernel<BN>, wm, xm, a);
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return p.pair ? cudaLaunchKernelEx(&cfg, gemm_fp8_pair_kernel, wm, xm, ym, a)
+                : cudaLaunchKernelEx(&cfg, gemm_fp8_small_kernel, wm, xm, ym, a);
 }
 
 }  // namespace
@@ -496,7 +855,12 @@ extern "C" int specb200_linear_fp8(const void* x, int64_t ldx, const float* x_sc
   const F8Plan p = plan_fp8(M, N, K);
   if (static_cast<int64_t>(p.m_tiles) * p.n_tiles > (1 << 30)) return specb200_set_error(SPECB200_ERR_ARG, "linear_fp8: M x N too large");
   CUtensorMap wm, xm;
-  if (!make_tmap_u8_2d(&wm, w, K, N, ldw, kFp8Group, p.bn) || !make_tmap_u8_2d(&xm, x, K, M, ldx, kFp8Group, p.box_rows))
+  if (!make_tmap_u8_2d(&wm, w, K, N, ldw, kFp8Group, kF8TileM) || !make_tmap_u8_2d(&xm, x, K, M, ldx, kFp8Group, p.box_rows))
+    return specb200_set_error(SPECB200_ERR_ARG, "linear_fp8: TMA descriptor");
+  CUtensorMap ym = {};
+  const int esize = out_f32 ? 4 : 2;
+  const bool y_rows16 = fp8_aligned(y, 16) && (ldy * esize) % 16 == 0;
+  if (p.splits == 1 && y_rows16 && !make_tmap_out_2d(&ym, y, out_f32 != 0, N, M, ldy * esize, 128 / esize, 32))
     return specb200_set_error(SPECB200_ERR_ARG, "linear_fp8: TMA descriptor");
   F8Args a = {};
   a.M = M;
@@ -514,10 +878,10 @@ extern "C" int specb200_linear_fp8(const void* x, int64_t ldx, const float* x_sc
   a.y = y;
   a.ldy = ldy;
   a.out_f32 = out_f32 ? 1 : 0;
-  a.vec_y = fp8_aligned(y, 16) && (ldy * (out_f32 ? 4 : 2)) % 16 == 0;
+  a.rows16 = y_rows16;
   a.status = status;
   cudaError_t e = cudaSuccess;
   if (status) e = cudaMemsetAsync(status, 0, sizeof(int32_t), s);
-  if (e == cudaSuccess) e = p.bn == 128 ? launch_fp8<128>(p, wm, xm, a, s) : launch_fp8<256>(p, wm, xm, a, s);
+  if (e == cudaSuccess) e = launch_fp8(p, wm, xm, ym, a, s);
   return e == cudaSuccess ? SPECB200_OK : specb200_set_error(SPECB200_ERR_CUDA, cudaGetErrorString(e));
 }

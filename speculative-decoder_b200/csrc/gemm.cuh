@@ -82,5 +82,8 @@ bool make_tmap_bf16_2d(CUtensorMap* map, const void* base, uint64_t inner, uint6
 // The same over bytes (e4m3 operands), rows `pitch` bytes apart.
 bool make_tmap_u8_2d(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer, uint64_t pitch,
                      uint32_t box_inner, uint32_t box_outer);
+// For storing bf16 or fp32 tiles whose rows are 128 bytes (128-byte swizzle), rows `pitch` bytes apart.
+bool make_tmap_out_2d(CUtensorMap* map, void* base, bool f32, uint64_t inner, uint64_t outer, uint64_t pitch,
+                      uint32_t box_inner, uint32_t box_outer);
 
 }  // namespace specb200
