@@ -10,7 +10,6 @@ library or without a CUDA device every entry point raises.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 from pathlib import Path
 
@@ -112,6 +111,16 @@ def lib() -> ctypes.CDLL:
     return _lib
 
 
+def torch_ops():
+    """The extension module specb200._torch_ops. Raises if it has not been built."""
+    try:
+        from specb200 import _torch_ops
+    except ImportError as e:
+        raise RuntimeError(f"specb200/_torch_ops.so cannot be loaded ({e}): build it with `python -m specb200.build` "
+                           "(the engine has no CPU fallback)") from e
+    return _torch_ops
+
+
 class ZeroDraftMass(ValueError):
     pass
 
@@ -160,20 +169,6 @@ def ptr(t: torch.Tensor | None) -> int | None:
 
 def stream_ptr(device: torch.device | None = None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
-
-
-def raw_stream(device: torch.device) -> int:
-    """stream_ptr without the Stream object in between (0.1 instead of 2.3 us of host time per call,
-    beside a launch of 4)."""
-    return torch._C._cuda_getCurrentRawStream(device.index)
-
-
-_HERE = contextlib.nullcontext()
-
-
-def on_device(device: torch.device):
-    """Makes `device` current for a launch (a stream takes launches from its own device only)."""
-    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 class Workspace:

@@ -1,4 +1,5 @@
-"""In-tree build of libspecb200.so (the CUDA kernels + C ABI) for sm_100a.
+"""In-tree build of libspecb200.so (the CUDA kernels + C ABI) for sm_100a, and of _torch_ops.so, the
+extension module through which specb200.ops calls the 8-bit operators with torch tensors.
 
     python -m specb200.build        (with speculative-decoder_b200/ on sys.path)
 
@@ -20,6 +21,8 @@ ROOT = PKG.parent
 CSRC = ROOT / "csrc"
 INCLUDE = ROOT.parent / "include"
 LIB = PKG / "libspecb200.so"
+TORCH_OPS_SRC = CSRC / "torch_ops.cpp"
+TORCH_OPS = PKG / "_torch_ops.so"
 OBJ_DIR = PKG / "_obj"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -49,7 +52,43 @@ def up_to_date() -> bool:
     return all(p.stat().st_mtime <= built for p in _inputs())
 
 
+def _run(cmd: list[str], what: str, verbose: bool) -> None:
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"{what} failed:\n{res.stdout}\n{res.stderr}")
+
+
+def build_torch_ops(verbose: bool = False, force: bool = False) -> Path:
+    """The extension module, linked to libspecb200.so beside it and to the installed torch."""
+    inputs = [TORCH_OPS_SRC, INCLUDE / "specb200.h"]
+    if not force and TORCH_OPS.exists() and all(p.stat().st_mtime <= TORCH_OPS.stat().st_mtime for p in inputs):
+        return TORCH_OPS
+    import sysconfig
+
+    import torch
+
+    base = Path(torch.__file__).resolve().parent
+    cuda = Path(nvcc()).resolve().parents[1]
+    tmp = TORCH_OPS.with_suffix(".so.tmp")
+    _run([shutil.which("g++") or "g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
+          f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+          *(f"-I{p}" for p in (INCLUDE, sysconfig.get_paths()["include"], cuda / "include")),
+          *(f"-isystem{p}" for p in (base / "include", base / "include" / "torch" / "csrc" / "api" / "include")),
+          str(TORCH_OPS_SRC), "-o", str(tmp), f"-L{PKG}", "-l:libspecb200.so", f"-L{base / 'lib'}", "-lc10", "-lc10_cuda",
+          "-ltorch_cpu", "-ltorch", "-ltorch_python", "-Wl,-rpath,$ORIGIN"], "_torch_ops", verbose)
+    os.replace(tmp, TORCH_OPS)
+    return TORCH_OPS
+
+
 def build(verbose: bool = False, force: bool = False) -> Path:
+    build_lib(verbose, force)
+    build_torch_ops(verbose, force)
+    return LIB
+
+
+def build_lib(verbose: bool = False, force: bool = False) -> Path:
     if not force and up_to_date():
         return LIB
     OBJ_DIR.mkdir(exist_ok=True)

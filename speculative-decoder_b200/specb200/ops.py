@@ -157,42 +157,16 @@ def verify_ids(ctx: torch.Tensor, ctx_len: torch.Tensor, draft: torch.Tensor, ou
 
 
 # ---------------------------------------------------------------- 8-bit operands
-FP8 = torch.float8_e4m3fn
-FP8_GROUP = 128  # columns (and, for weights, rows) that share a scale
+_torch_ops = None
 
 
-def _same_device(where: str, first: torch.Tensor, *others: torch.Tensor | None) -> torch.device:
-    _ffi.require_cuda(first, where)
-    for t in others:
-        if t is not None and t.device != first.device:
-            raise ValueError(f"{where}: tensors on {first.device} and {t.device}")
-    return first.device
-
-
-def _rows(x: torch.Tensor) -> torch.Tensor:
-    """[..., K] as [M, K] with consecutive columns; rows may be any pitch apart."""
-    if x.dim() == 0:
-        raise ValueError("expected rows, got a scalar")
-    if x.dim() != 2:
-        x = x.reshape(-1, x.shape[-1]) if x.numel() else x.new_empty((x.shape[:-1].numel(), x.shape[-1]))
-    return x if x.stride(1) == 1 and x.stride(0) >= x.shape[1] else x.contiguous()
-
-
-def _pitch(rows: torch.Tensor) -> int:
-    """Elements from row to row (of a single row, which may have any stride: a pitch that fits it)."""
-    return rows.stride(0) if rows.shape[0] != 1 else (rows.shape[1] + 15) // 16 * 16
-
-
-def _fp8_out(m: int, k: int, block_rows: int, device: torch.device) -> tuple[torch.Tensor, torch.Tensor]:
-    """Room for e4m3 rows that start on 16-byte boundaries (linear_fp8 loads them by TMA), and scales."""
-    q = torch.empty(m, (k + 15) // 16 * 16, dtype=FP8, device=device)
-    scales = torch.empty(-(-m // block_rows), -(-k // FP8_GROUP), dtype=torch.float32, device=device)
-    return (q if k % 16 == 0 else q[:, :k]), scales
-
-
-def _shaped(lead: torch.Size, *parts: torch.Tensor) -> tuple[torch.Tensor, ...]:
-    """Row outputs with the input's leading dimensions."""
-    return parts if len(lead) == 1 else tuple(p.view(*lead, p.shape[-1]) for p in parts)
+def _ext():
+    """The extension module that checks arguments, allocates outputs and launches for these operators
+    (csrc/torch_ops.cpp)."""
+    global _torch_ops
+    if _torch_ops is None:
+        _torch_ops = _ffi.torch_ops()
+    return _torch_ops
 
 
 def quantize_fp8(x: torch.Tensor, block_rows: int = 1) -> tuple[torch.Tensor, torch.Tensor]:
@@ -200,20 +174,7 @@ def quantize_fp8(x: torch.Tensor, block_rows: int = 1) -> tuple[torch.Tensor, to
     q = e4m3(x / s). block_rows 1 (activations): a scale per row and 128 columns,
     [..., ceil(K / 128)]. block_rows 128 (weights, x [N, K]): one per 128 x 128 block,
     [ceil(N / 128), ceil(K / 128)]. q's rows are padded to 16 bytes in memory."""
-    dev = _same_device("quantize_fp8", x)
-    if block_rows not in (1, FP8_GROUP):
-        raise ValueError(f"quantize_fp8: block_rows is 1 or {FP8_GROUP}, not {block_rows}")
-    if block_rows != 1 and x.dim() != 2:
-        raise ValueError(f"quantize_fp8: blocks of {FP8_GROUP} rows need a matrix, got shape {tuple(x.shape)}")
-    code = _dtype_code(x.dtype)
-    rows = _rows(x)
-    m, k = rows.shape
-    q, scales = _fp8_out(m, k, block_rows, dev)
-    with _ffi.on_device(dev):
-        rc = lib().specb200_quantize_fp8(code, ptr(rows), _pitch(rows), m, k, block_rows, ptr(q), q.stride(0),
-                                         ptr(scales), _ffi.raw_stream(dev))
-    raise_for(rc, "specb200_quantize_fp8")
-    return (q, scales) if x.dim() == 2 else _shaped(x.shape[:-1], q, scales)
+    return _ext().quantize_fp8(x, block_rows)
 
 
 def rmsnorm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float,
@@ -221,57 +182,13 @@ def rmsnorm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float,
     """RMSNorm with an 8-bit output: (q, scales) of weight * h / sqrt(mean(h^2) + eps) for h = x
     [..., H], the values of quantize_fp8 on the fp32 product. With delta, the residual update
     h = x + delta (rounded to x's dtype) comes first and the result is (q, scales, h)."""
-    dev = _same_device("rmsnorm_fp8", x, weight, delta)
-    code = _dtype_code(x.dtype)
-    if weight.shape != x.shape[-1:] or weight.dtype != x.dtype:
-        raise ValueError(f"rmsnorm_fp8: weight is {weight.dtype} {tuple(weight.shape)} for x {x.dtype} {tuple(x.shape)}")
-    if delta is not None and (delta.shape != x.shape or delta.dtype != x.dtype):
-        raise ValueError(f"rmsnorm_fp8: delta is {delta.dtype} {tuple(delta.shape)} for x {x.dtype} {tuple(x.shape)}")
-    rows = _rows(x)
-    m, k = rows.shape
-    weight = weight.contiguous()
-    q, scales = _fp8_out(m, k, 1, dev)
-    d = h = None
-    if delta is not None:
-        d = _rows(delta)
-        h = torch.empty(m, k, dtype=x.dtype, device=dev)
-    with _ffi.on_device(dev):
-        rc = lib().specb200_rmsnorm_fp8(code, ptr(rows), _pitch(rows), ptr(d), 0 if d is None else _pitch(d),
-                                        ptr(weight), m, k, eps, ptr(h), k, ptr(q), q.stride(0), ptr(scales),
-                                        _ffi.raw_stream(dev))
-    raise_for(rc, "specb200_rmsnorm_fp8")
-    out = (q, scales) if h is None else (q, scales, h)
-    return out if x.dim() == 2 else _shaped(x.shape[:-1], *out)
+    return _ext().rmsnorm_fp8(x, weight, eps, delta)
 
 
 def silu_mul_fp8(gate_up: torch.Tensor, packed: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
     """(q, scales) of silu(gate) * up for gate_up [..., 2 I]: the gate columns, then the up columns,
     or with packed 64-column groups of gate then up (the order of the engine's packed gate/up weights)."""
-    dev = _same_device("silu_mul_fp8", gate_up)
-    code = _dtype_code(gate_up.dtype)
-    rows = _rows(gate_up)
-    m, both = rows.shape
-    if both % (128 if packed else 2):
-        raise ValueError(f"silu_mul_fp8: {both} columns are not gate and up{' in groups of 64' if packed else ''}")
-    q, scales = _fp8_out(m, both // 2, 1, dev)
-    with _ffi.on_device(dev):
-        rc = lib().specb200_silu_mul_fp8(code, ptr(rows), _pitch(rows), m, both // 2, int(packed), ptr(q),
-                                         q.stride(0), ptr(scales), _ffi.raw_stream(dev))
-    raise_for(rc, "specb200_silu_mul_fp8")
-    return (q, scales) if gate_up.dim() == 2 else _shaped(gate_up.shape[:-1], q, scales)
-
-
-def _fp8_operand(x: torch.Tensor, what: str) -> torch.Tensor:
-    """[..., K] e4m3 as rows that TMA can load: 16-byte boundaries, copied there if need be."""
-    if x.dtype != FP8:
-        raise ValueError(f"linear_fp8: {what} is {x.dtype}, not {FP8}")
-    rows = _rows(x)
-    if _pitch(rows) % 16 or rows.data_ptr() % 16:
-        m, k = rows.shape
-        held = torch.empty(m, (k + 15) // 16 * 16, dtype=torch.uint8, device=x.device)
-        held[:, :k].copy_(rows.view(torch.uint8))
-        rows = held.view(FP8)[:, :k]
-    return rows
+    return _ext().silu_mul_fp8(gate_up, packed)
 
 
 def linear_fp8(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor,
@@ -279,26 +196,6 @@ def linear_fp8(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scale
     """x [..., K] @ w[N, K]^T on e4m3 operands with a scale per 128 of K (quantize_fp8, rmsnorm_fp8,
     silu_mul_fp8: x_scales [..., ceil(K / 128)]) and per 128 x 128 block of w (quantize_fp8 with
     block_rows 128: w_scales [ceil(N / 128), ceil(K / 128)]); fp32 accumulation, bf16 or fp32 out.
-    check reads the device status back (and waits for the stream)."""
-    dev = _same_device("linear_fp8", x, x_scales, w, w_scales)
-    if x.dim() == 0 or w.dim() != 2 or x.shape[-1] != w.shape[1]:
-        raise ValueError(f"linear_fp8: x {tuple(x.shape)} and w {tuple(w.shape)} do not multiply")
-    rows, w = _fp8_operand(x, "x"), _fp8_operand(w, "w")
-    m, k = rows.shape
-    n = w.shape[0]
-    groups = -(-k // FP8_GROUP)
-    if x_scales.shape != (*x.shape[:-1], groups) or w_scales.shape != (-(-n // FP8_GROUP), groups):
-        raise ValueError(f"linear_fp8: scales {tuple(x_scales.shape)} and {tuple(w_scales.shape)} for x "
-                         f"{tuple(x.shape)}, w {tuple(w.shape)}: one per {FP8_GROUP} of K and {FP8_GROUP} x {FP8_GROUP}")
-    if x_scales.dtype != torch.float32 or w_scales.dtype != torch.float32:
-        raise ValueError(f"linear_fp8: scales are float32, not {x_scales.dtype} and {w_scales.dtype}")
-    x_scales, w_scales = x_scales.contiguous(), w_scales.contiguous()
-    y = torch.empty(m, n, dtype=torch.float32 if out_f32 else torch.bfloat16, device=dev)
-    status = torch.empty(1, dtype=torch.int32, device=dev) if check else None
-    with _ffi.on_device(dev):
-        rc = lib().specb200_linear_fp8(ptr(rows), _pitch(rows), ptr(x_scales), ptr(w), _pitch(w), ptr(w_scales), m, n, k,
-                                       int(out_f32), ptr(y), n, ptr(status), _ffi.raw_stream(dev))
-    raise_for(rc, "specb200_linear_fp8")
-    if check:
-        _ffi.check_status(status, "linear_fp8")
-    return y if x.dim() == 2 else y.view(*x.shape[:-1], n)
+    Operands whose rows are not on 16-byte boundaries are copied there first. check reads the device
+    status back (and waits for the stream)."""
+    return _ext().linear_fp8(x, x_scales, w, w_scales, out_f32, check)
