@@ -13,6 +13,35 @@
 namespace specb200 {
 namespace {
 
+// Two fp32 values in a register pair, one instruction for both: these kernels run next to the
+// power limit, where every instruction saved is clock rate gained.
+typedef unsigned long long f32x2;
+SPECB200_DEVINL f32x2 pack2(float lo, float hi) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+SPECB200_DEVINL float2 unpack2(f32x2 v) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+  return f;
+}
+SPECB200_DEVINL f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+SPECB200_DEVINL f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+SPECB200_DEVINL f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
 // Sixteen consecutive elements of a row, in the form they have in memory. align: every row starts
 // on a boundary of that many bytes: 32 takes 256-bit loads, 16 takes 128-bit ones, less one load
 // per element.
@@ -56,48 +85,58 @@ SPECB200_DEVINL void load16(Raw16<T>& r, const T* p, int valid, int align) {
   }
 }
 template <typename T>
-SPECB200_DEVINL void unpack16(const Raw16<T>& r, float (&f)[16]) {
-  if constexpr (sizeof(T) == 2) {
+SPECB200_DEVINL void unpack16(const Raw16<T>& r, f32x2 (&f)[8]) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      f[2 * i] = __uint_as_float(r.v[i] << 16);
-      f[2 * i + 1] = __uint_as_float(r.v[i] & 0xffff0000u);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(r.v[i]);
+  for (int i = 0; i < 8; ++i) {
+    if constexpr (sizeof(T) == 2)
+      f[i] = pack2(__uint_as_float(r.v[i] << 16), __uint_as_float(r.v[i] & 0xffff0000u));
+    else
+      f[i] = pack2(__uint_as_float(r.v[2 * i]), __uint_as_float(r.v[2 * i + 1]));
   }
 }
+// Rounded to T, in memory's form.
 template <typename T>
-SPECB200_DEVINL void store16(T* p, int valid, int align, const float (&f)[16]) {
+SPECB200_DEVINL Raw16<T> round16(const f32x2 (&f)[8]) {
+  Raw16<T> r;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float2 v = unpack2(f[i]);
+    if constexpr (sizeof(T) == 2) {
+      const __nv_bfloat162 b = __floats2bfloat162_rn(v.x, v.y);
+      r.v[i] = *reinterpret_cast<const uint32_t*>(&b);
+    } else {
+      r.v[2 * i] = __float_as_uint(v.x);
+      r.v[2 * i + 1] = __float_as_uint(v.y);
+    }
+  }
+  return r;
+}
+template <typename T>
+SPECB200_DEVINL void store16(T* p, int valid, int align, const Raw16<T>& r) {
   constexpr int kWords = 4 * sizeof(T);
   if (align >= 16 && valid >= 16) {
-    uint32_t u[kWords];
-#pragma unroll
-    for (int i = 0; i < kWords; ++i) {
-      if constexpr (sizeof(T) == 2) {
-        const __nv_bfloat162 b = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
-        u[i] = *reinterpret_cast<const uint32_t*>(&b);
-      } else {
-        u[i] = __float_as_uint(f[i]);
-      }
-    }
 #pragma unroll
     for (int i = 0; i < kWords; i += 4)
-      reinterpret_cast<uint4*>(p)[i / 4] = make_uint4(u[i], u[i + 1], u[i + 2], u[i + 3]);
+      reinterpret_cast<uint4*>(p)[i / 4] = make_uint4(r.v[i], r.v[i + 1], r.v[i + 2], r.v[i + 3]);
     return;
   }
 #pragma unroll
-  for (int i = 0; i < 16; ++i)
-    if (i < valid) p[i] = from_f32<T>(f[i]);
+  for (int i = 0; i < 16; ++i) {
+    if constexpr (sizeof(T) == 2) {
+      if (i < valid) reinterpret_cast<unsigned short*>(p)[i] = static_cast<unsigned short>(r.v[i / 2] >> (16 * (i & 1)));
+    } else {
+      if (i < valid) reinterpret_cast<uint32_t*>(p)[i] = r.v[i];
+    }
+  }
 }
 // e4m3(f * inv), 16 of a row.
-SPECB200_DEVINL void store_q16(uint8_t* p, int valid, int align, const float (&f)[16], float inv) {
+SPECB200_DEVINL void store_q16(uint8_t* p, int valid, int align, const f32x2 (&f)[8], float inv) {
+  const f32x2 inv2 = pack2(inv, inv);
   uint32_t v[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(f[4 * i] * inv, f[4 * i + 1] * inv), __NV_SATFINITE, __NV_E4M3);
-    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(f[4 * i + 2] * inv, f[4 * i + 3] * inv), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(unpack2(mul2(f[2 * i], inv2)), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(unpack2(mul2(f[2 * i + 1], inv2)), __NV_SATFINITE, __NV_E4M3);
     v[i] = lo | (hi << 16);
   }
   if (align >= 16 && valid >= 16) {
@@ -109,10 +148,13 @@ SPECB200_DEVINL void store_q16(uint8_t* p, int valid, int align, const float (&f
     if (i < valid) p[i] = static_cast<uint8_t>(v[i / 4] >> (8 * (i & 3)));
 }
 
-SPECB200_DEVINL float max_mag16(const float (&f)[16]) {
+SPECB200_DEVINL float max_mag16(const f32x2 (&f)[8]) {
   float m = 0.f;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) m = max_mag(m, f[i]);
+  for (int i = 0; i < 8; ++i) {
+    const float2 v = unpack2(f[i]);
+    m = max_mag(max_mag(m, v.x), v.y);
+  }
   return m;
 }
 // Maximum over the 8 lanes that hold a group.
@@ -122,16 +164,20 @@ SPECB200_DEVINL float octet_max(float m) {
   return m;
 }
 
-// silu(g) * u = g u / (1 + e^-g). The exponential is 2^t with t = -g log2(e), whose rounding is
-// carried along (2^(hi + lo) = 2^hi (1 + lo ln 2)): without it a far gate loses |g| 2^-24.
-SPECB200_DEVINL float silu_mul(float g, float u) {
-  constexpr float kLog2e = 1.44269504f, kLn2 = 0.69314718f;
-  const float hi = -g * kLog2e, lo = fmaf(-g, kLog2e, -hi);
-  float e, s;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(hi));
-  const float d = 1.f + (isfinite(hi) ? fmaf(e, lo * kLn2, e) : e);
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(d));
-  return g * s * u;
+// silu(g) * u = g u / (1 + 2^(-g log2 e)) for a pair. The exponent is rounded to fp32, which leaves
+// |g| 2^-23 in the exponential: nothing next to the 1 for positive gates, and for negative ones a
+// relative error that grows as the value itself dies away. Where the exponential overflows its
+// reciprocal is zero; an infinite gate gives what the formula gives (inf u, or NaN).
+SPECB200_DEVINL f32x2 silu_mul2(f32x2 g, f32x2 u) {
+  constexpr float kLog2e = 1.44269504f;
+  const float2 t = unpack2(mul2(g, pack2(-kLog2e, -kLog2e)));
+  float2 e, s;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(t.x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(t.y));
+  const float2 d = unpack2(add2(pack2(e.x, e.y), pack2(1.f, 1.f)));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s.x) : "f"(d.x));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s.y) : "f"(d.y));
+  return mul2(mul2(g, pack2(s.x, s.y)), u);
 }
 
 struct RowArgs {
@@ -165,18 +211,18 @@ __global__ void __launch_bounds__(kRowThreads, sizeof(T) == 2 ? 8 : 5) quantize_
   const T* xr = static_cast<const T*>(a.x) + row * a.ldx;
   pdl_wait();
   Raw16<T> raw;
-  float y[16];
+  f32x2 y[8];
   if constexpr (kSilu) {
     // packed: feature j is gate column 128 (j / 64) + j % 64, its up column 64 further on
     const int gate = a.packed ? ((col >> 6) << 7) + (col & 63) : col;
     Raw16<T> raw_up;
     load16<T>(raw, xr + gate, valid, a.vec_in);
     load16<T>(raw_up, xr + gate + (a.packed ? 64 : a.K), valid, a.vec_in);
-    float up[16];
+    f32x2 up[8];
     unpack16<T>(raw, y);
     unpack16<T>(raw_up, up);
 #pragma unroll
-    for (int j = 0; j < 16; ++j) y[j] = silu_mul(y[j], up[j]);
+    for (int j = 0; j < 8; ++j) y[j] = silu_mul2(y[j], up[j]);
   } else {
     load16<T>(raw, xr + col, valid, a.vec_in);
     unpack16<T>(raw, y);
@@ -209,7 +255,7 @@ __global__ void __launch_bounds__(kRowThreads, sizeof(T) == 2 ? 3 : 2) quantize_
   float m = 0.f;
 #pragma unroll
   for (int p = 0; p < kPass; ++p) {
-    float y[16];
+    f32x2 y[8];
     unpack16<T>(x[p], y);
     m = max_nan(m, max_mag16(y));
   }
@@ -223,7 +269,7 @@ __global__ void __launch_bounds__(kRowThreads, sizeof(T) == 2 ? 3 : 2) quantize_
   const float inv = kE4m3Max / amax;
 #pragma unroll
   for (int p = 0; p < kPass; ++p) {
-    float y[16];
+    f32x2 y[8];
     unpack16<T>(x[p], y);
     if (r0 + p * kLanes < rows && valid > 0) store_q16(qp + p * kLanes * a.ldq, valid, a.vec_out, y, inv);
   }
@@ -297,17 +343,21 @@ __global__ void __launch_bounds__(kChunks == 4 ? 512 : 256, kNormCtas<T, kChunks
     load16<T>(w[c], static_cast<const T*>(a.weight) + col0 + c * pitch, a.H - (col0 + c * pitch), a.vec_w);
   for (int parity = 0; base < a.M; base += step, parity ^= 1) {
     const int64_t row = base + team;
-    float f[kChunks][16], m[kChunks];
-    float ss = 0.f;
+    f32x2 f[kChunks][8];
+    float m[kChunks], ss = 0.f;
     if constexpr (!kAhead) load_row(row);
 #pragma unroll
     for (int c = 0; c < kChunks; ++c) {
       unpack16<T>(x[c], f[c]);
       if constexpr (kDelta) {
-        float g[16];
+        f32x2 g[8];
         unpack16<T>(d[c], g);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) f[c][i] = round_to<T>(f[c][i] + g[i]);
+        for (int i = 0; i < 8; ++i) f[c][i] = add2(f[c][i], g[i]);
+        x[c] = round16<T>(f[c]);
+        const int col = col0 + c * pitch, valid = valid_of(row, c);
+        if (valid > 0) store16<T>(static_cast<T*>(a.h) + row * a.ldh + col, valid, a.vec_h, x[c]);
+        unpack16<T>(x[c], f[c]);
       }
     }
     if constexpr (kAhead) {
@@ -315,18 +365,15 @@ __global__ void __launch_bounds__(kChunks == 4 ? 512 : 256, kNormCtas<T, kChunks
     }
 #pragma unroll
     for (int c = 0; c < kChunks; ++c) {
-      const int col = col0 + c * pitch, valid = valid_of(row, c);
-      if constexpr (kDelta) {
-        if (valid > 0) store16<T>(static_cast<T*>(a.h) + row * a.ldh + col, valid, a.vec_h, f[c]);
-      }
-      float g[16], part = 0.f;
+      f32x2 g[8], part = pack2(0.f, 0.f);
       unpack16<T>(w[c], g);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        part = fmaf(f[c][i], f[c][i], part);
-        f[c][i] *= g[i];
+      for (int i = 0; i < 8; ++i) {
+        part = fma2(f[c][i], f[c][i], part);
+        f[c][i] = mul2(f[c][i], g[i]);
       }
-      ss += part;
+      const float2 sums = unpack2(part);
+      ss += sums.x + sums.y;
       m[c] = octet_max(max_mag16(f[c]));
     }
 #pragma unroll
@@ -353,7 +400,7 @@ __global__ void __launch_bounds__(kChunks == 4 ? 512 : 256, kNormCtas<T, kChunks
       const bool cancels = amax > kFp8MinAmax && amax <= 3.402823466e38f && m[c] >= kFp8MinAmax;
       if (!cancels) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) f[c][i] *= r;
+        for (int i = 0; i < 8; ++i) f[c][i] = mul2(f[c][i], pack2(r, r));
       }
       if (valid > 0) {
         store_q16(a.q + row * a.ldq + col, valid, a.vec_q, f[c], kE4m3Max / (cancels ? m[c] : amax));
