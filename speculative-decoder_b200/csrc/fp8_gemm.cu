@@ -18,6 +18,7 @@
 //   instead of 48, and holds 128 tokens of the accumulators.
 #include <algorithm>
 #include <atomic>
+#include <cstdlib>
 
 #include "fp8.cuh"
 #include "gemm.cuh"
@@ -231,11 +232,12 @@ SPECB200_DEVINL void store_quad(const F8Args& a, int64_t at, int valid, const fl
     if (i < valid) p[i] = __float2bfloat16_rn(v[i]);
 }
 
-// A scale, loaded here and not where the compiler would rather have it: a group ahead of its use.
-SPECB200_DEVINL float load_scale(const float* p) {
-  float v;
-  asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(v) : "l"(p));
-  return v;
+// Two fp32 accumulators in a register pair: d += {t0, t1} * f in one instruction.
+typedef unsigned long long f32x2;
+SPECB200_DEVINL void add2(f32x2& d, uint32_t t0, uint32_t t1, float f) {
+  asm("{\n\t.reg .b64 t, g;\n\tmov.b64 t, {%1, %2};\n\tmov.b64 g, {%3, %3};\n\tfma.rn.f32x2 %0, t, g, %0;\n\t}"
+      : "+l"(d)
+      : "r"(t0), "r"(t1), "f"(f));
 }
 
 // Four bytes to shared memory, and an arrival at `bar` once this thread's copies so far are there.
@@ -313,25 +315,44 @@ SPECB200_DEVINL void store_warp_tile(const F8Args& a, const CUtensorMap& y_map, 
 }
 
 // ------------------------------------------------------------------------------ small tiles
+// The scales of one group: of a CTA's 128 tokens and of the tile's weight blocks (two for a pair).
+struct F8Scales {
+  float x[kF8TileM], w[4];
+};
 struct F8SmallBarriers {
-  uint64_t full[kF8MaxStages], done[kF8MaxStages], tempty[2];
+  uint64_t full[kF8MaxStages], done[kF8MaxStages], sfull[kF8MaxStages + 4], tempty[4];
   uint32_t tmem_holder;
   int abort_flag;
 };
 
-// Warps 0-7 read back (w on TMEM lane quarter w % 4, columns 64 (w / 4)..), warp 8 issues TMA, warp 9
-// tcgen05.mma. A stage's `done` barrier frees its operands and completes its accumulator.
-__global__ void __launch_bounds__(kF8SmallThreads, 2)
+// One warp's copy of a group's scales to shared memory; `filled` (32 arrivals) completes when they
+// are there. sx, sw: this lane's first token's and weight block's scale of the group.
+SPECB200_DEVINL void copy_scales(F8Scales& to, uint64_t* filled, const float* sx, const float* sw, int64_t pitch32,
+                                 int tokens, bool live_w, int lane) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (32 * i + lane < tokens) copy_async_4(&to.x[32 * i + lane], sx + i * pitch32);
+  if (live_w) copy_async_4(&to.w[lane], sw);
+  copy_async_arrive(filled);
+}
+
+// Warps 0-7 read back (w on TMEM lane quarter w % 4, columns 64 (w / 4)..), warp 8 issues TMA and
+// fetches scales, warp 9 tcgen05.mma. A stage's `done` barrier frees its operands and completes its
+// accumulator. Small calls are bound by latency, so loads start before TMEM is allocated: the
+// epilogue learns of the allocation through the first `done`.
+template <int kPerSm>
+__global__ void __launch_bounds__(kF8SmallThreads, kPerSm)
     gemm_fp8_small_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map,
                           const __grid_constant__ CUtensorMap y_map, F8Args a) {
   constexpr int kCols = 64;                  // features per epilogue thread
-  constexpr int kLd = 16;                    // accumulator columns read back at a time (what registers allow)
+  constexpr int kBufs = kPerSm == 1 ? 4 : 2; // TMEM buffers
+  constexpr int kLd = kPerSm == 1 ? 32 : 16; // accumulator columns read back at a time (what registers allow)
   constexpr int kPitch = kF8Block + 4;       // partial tile's row pitch (floats)
-  // the ring (1024-byte swizzle atoms), which ends up holding the output; then the barriers
+  // the ring (1024-byte swizzle atoms), which ends up holding the output; barriers; scales
   extern __shared__ __align__(1024) uint8_t smem[];
   F8SmallBarriers& bars = *reinterpret_cast<F8SmallBarriers*>(smem + a.ring_bytes);
-  uint64_t *full = bars.full, *done = bars.done, *tempty = bars.tempty;
-  uint32_t& tmem_holder = bars.tmem_holder;
+  F8Scales* scales = reinterpret_cast<F8Scales*>(&bars + 1);  // stages + kBufs of them
+  uint64_t *full = bars.full, *done = bars.done, *sfull = bars.sfull, *tempty = bars.tempty;
   int& abort_flag = bars.abort_flag;
   const uint32_t stage_bytes = kF8TileBytes + a.x_bytes;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -342,18 +363,15 @@ __global__ void __launch_bounds__(kF8SmallThreads, 2)
       mbar_init(&full[i], 1);
       mbar_init(&done[i], 1);
     }
-    for (int i = 0; i < 2; ++i) mbar_init(&tempty[i], kF8EpiWarps);
+    for (uint32_t i = 0; i < stages + kBufs; ++i) mbar_init(&sfull[i], 32);
+    for (int i = 0; i < kBufs; ++i) mbar_init(&tempty[i], kF8EpiWarps);
     abort_flag = 0;
     fence_mbar_init();
+  } else if (warp == 8 && lane == 0) {
+    tma_prefetch_desc(&w_map);
+    tma_prefetch_desc(&x_map);
   }
-  if (warp == 9) f8_tmem_alloc<false>(&tmem_holder, 2 * kF8Block);
-  tc_fence_before();
   __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = tmem_holder;
-  // Only now may the next kernel's CTAs start: one that allocated TMEM before this CTA and then
-  // waited for it would keep it from ever starting.
-  pdl_launch_dependents();
 
   // a cluster is one tile, its CTAs the splits of K
   const int splits = a.splits, split = static_cast<int>(blockIdx.x) % splits, tile = static_cast<int>(blockIdx.x) / splits;
@@ -362,88 +380,154 @@ __global__ void __launch_bounds__(kF8SmallThreads, 2)
   const int kb1 = static_cast<int>(static_cast<int64_t>(a.kblocks) * (split + 1) / splits);
 
   if (warp == 8) {
-    if (lane == 0) {
-      tma_prefetch_desc(&w_map);
-      tma_prefetch_desc(&x_map);
-      pdl_wait();
-      uint32_t st = 0, phase = 0, issued = 0;
-      bool ok = true;
-      for (int kb = kb0; kb < kb1; ++kb) {
-        ok = mbar_wait_bounded(&done[st], phase ^ 1, a.status, &abort_flag);
-        if (!ok) break;
+    pdl_wait();
+    const float* sx = a.xs + static_cast<int64_t>(tile_m + lane) * a.kblocks + kb0;
+    const float* sw = a.ws + static_cast<int64_t>(tile_n / kF8Block) * a.kblocks + kb0;
+    const int64_t pitch32 = static_cast<int64_t>(32) * a.kblocks;
+    const int tokens = a.M - tile_m, groups = kb1 - kb0;
+    auto load = [&](int g, uint32_t st) {
+      if (lane == 0) {
         uint8_t* s = smem + st * stage_bytes;
         mbar_arrive_expect_tx(&full[st], stage_bytes);
-        tma_load_2d(s, &w_map, &full[st], kb * kFp8Group, tile_n);
-        tma_load_2d(s + kF8TileBytes, &x_map, &full[st], kb * kFp8Group, tile_m);
-        if (issued < stages) ++issued;
-        if (++st == stages) { st = 0; phase ^= 1; }
+        tma_load_2d(s, &w_map, &full[st], (kb0 + g) * kFp8Group, tile_n);
+        tma_load_2d(s + kF8TileBytes, &x_map, &full[st], (kb0 + g) * kFp8Group, tile_m);
       }
-      // Tail: the last use of every stage is done (so no commit arrives after the exit), or, where
-      // a wait gave up, at least every copy in flight has landed.
-      for (uint32_t i = 0; i < issued; ++i) {
-        if (st == 0) { st = stages; phase ^= 1; }
-        --st;
-        if (ok) ok = mbar_wait_bounded(&done[st], phase, a.status, &abort_flag);
-        if (!ok) mbar_wait_bounded(&full[st], phase, a.status, nullptr);
-      }
+    };
+    auto fetch = [&](int g, uint32_t slot) {
+      copy_scales(scales[slot], &sfull[slot], sx + g, sw + g, pitch32, tokens, lane == 0, lane);
+    };
+    // The ring's first filling waits for nothing: operands first, then their scales. A slot of
+    // scales is used again kBufs groups later than a stage (see gemm_fp8_pair_kernel).
+    const int first = min(groups, static_cast<int>(stages));
+    for (int g = 0; g < first; ++g) load(g, g);
+    for (int g = 0; g < first; ++g) fetch(g, g);
+    uint32_t st = 0, phase = 0, slot = stages;
+    bool ok = true;
+    for (int g = first; g < groups; ++g) {
+      ok = wait_warp(&done[st], phase, a.status, &abort_flag);
+      if (!ok) break;
+      load(g, st);
+      fetch(g, slot);
+      if (++st == stages) { st = 0; phase ^= 1; }
+      if (++slot == stages + kBufs) slot = 0;
     }
+    // Tail: the last use of every stage is done (so no commit arrives after the exit), or, where a
+    // wait gave up, at least every copy in flight has landed.
+    for (int i = 0; i < first; ++i) {
+      const uint32_t s = first < static_cast<int>(stages) ? i : st, p = phase;
+      if (++st == stages) { st = 0; phase ^= 1; }
+      if (ok) ok = wait_warp(&done[s], p, a.status, &abort_flag);
+      if (!ok && lane == 0) mbar_wait_bounded(&full[s], p, a.status, nullptr);
+      __syncwarp();
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    pdl_launch_dependents();
   } else if (warp == 9) {
+    f8_tmem_alloc<false>(&bars.tmem_holder, kBufs * kF8Block);
+    __syncwarp();
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&bars.tmem_holder);
+    // Only from here on may the next kernel's CTAs start (each warp allows it once it knows of the
+    // allocation): one that allocated TMEM before this CTA and then waited for it would keep it
+    // from ever starting.
+    pdl_launch_dependents();
     constexpr uint32_t idesc = umma_idesc_e4m3(kF8TileM, kF8Block);
     const uint32_t leader = elect_leader();
     const uint64_t dw0 = umma_desc_sw128(smem_u32(smem)), dx0 = umma_desc_sw128(smem_u32(smem + kF8TileBytes));
     uint32_t st = 0, phase = 0, buf = 0, acc_phase = 0;
     for (int kb = kb0; kb < kb1; ++kb) {
-      if (!wait_warp(&tempty[buf], acc_phase ^ 1, a.status, &abort_flag) ||
-          !wait_warp(&full[st], phase, a.status, &abort_flag))
-        break;
+      if (!wait_warp<true>(&tempty[buf], acc_phase ^ 1, &full[st], phase, a.status, &abort_flag)) break;
       tc_fence_after();
       const uint64_t at = static_cast<uint64_t>(st * (stage_bytes >> 4));
       umma_group_e4m3<false>(leader, tmem + buf * kF8Block, dx0 + at, dw0 + at, idesc, &done[st]);
       if (++st == stages) { st = 0; phase ^= 1; }
-      buf ^= 1;
-      acc_phase ^= buf ^ 1;
+      if (++buf == kBufs) { buf = 0; acc_phase ^= 1; }
     }
   } else {
     pdl_wait();
     const int quarter = warp & 3, col0 = (warp >> 2) * kCols;
-    const uint32_t tbase = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + col0;
     const int m0 = tile_m + quarter * 32, n0 = tile_n + col0;
     const bool live = m0 < a.M && n0 < a.N;  // warps without outputs only keep step
-    const float* sx = a.xs + static_cast<int64_t>(min(m0 + lane, a.M - 1)) * a.kblocks;
-    const float* sw = a.ws + static_cast<int64_t>(tile_n / kF8Block) * a.kblocks;
     float acc[kCols];
 #pragma unroll
     for (int i = 0; i < kCols; ++i) acc[i] = 0.f;
-    float fx = live ? load_scale(sx + kb0) : 0.f, fw = live ? load_scale(sw + kb0) : 0.f;
-    uint32_t st = 0, phase = 0, buf = 0;
-    bool ok = true;
-    for (int kb = kb0; kb < kb1; ++kb) {
-      const float f = fx * fw;
-      if (live && kb + 1 < kb1) {
-        fx = load_scale(sx + kb + 1);
-        fw = load_scale(sw + kb + 1);
-      }
-      ok = wait_warp(&done[st], phase, a.status, &abort_flag);
-      if (!ok) break;
+    uint32_t st = 0, phase = 0, buf = 0, slot = 0, slot_phase = 0;
+    // A poll (`tried`) is issued early, its outcome looked at (`ready`) where it is needed.
+    auto try_ready = [&] { return mbar_try_wait(&done[st], phase) && mbar_try_wait(&sfull[slot], slot_phase); };
+    auto ready = [&](bool tried) {
+      const bool ok = __all_sync(0xffffffffu, tried) ||
+                      wait_warp<true>(&done[st], phase, &sfull[slot], slot_phase, a.status, &abort_flag);
       tc_fence_after();
-      if (live) {
+      return ok;
+    };
+    auto release = [&](uint32_t b) {  // this buffer is read: a later group may overwrite it
+      tc_fence_before();
+      if (lane == 0) mbar_arrive(&tempty[b]);
+    };
+    auto advance = [&] {
+      if (++st == stages) { st = 0; phase ^= 1; }
+      if (++slot == stages + kBufs) { slot = 0; slot_phase ^= 1; }
+      if (++buf == kBufs) buf = 0;
+    };
+    auto factor = [&] { return scales[slot].x[quarter * 32 + lane] * scales[slot].w[0]; };
+    bool ok = ready(try_ready());
+    const uint32_t tbase = ok ? *reinterpret_cast<volatile uint32_t*>(&bars.tmem_holder) + (static_cast<uint32_t>(quarter * 32) << 16) + col0 : 0;
+    pdl_launch_dependents();
+    int groups = kb1 - kb0;
+    if (!live) {
+      while (ok) {
+        release(buf);
+        advance();
+        if (--groups == 0) break;
+        ok = ready(try_ready());
+      }
+    } else if constexpr (kPerSm == 1) {
+      // 32 columns come back at a time, the next ones and the next group's poll on their way while
+      // the last ones are added: 
+      uint32_t r0[32], r1[32];
+      auto add = [&](int c, const uint32_t (&r)[32], float f) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) acc[c + i] = fmaf(__uint_as_float(r[i]), f, acc[c + i]);
+      };
+      if (ok) {
+        float f = factor();
+        tmem_ld<32>(tbase + buf * kF8Block, r0);
+        for (;;) {
+          tmem_ld_wait();
+          tmem_ld<32>(tbase + buf * kF8Block + 32, r1);
+          const uint32_t last = buf;
+          advance();
+          const bool more = --groups > 0, tried = more && try_ready();
+          add(0, r0, f);
+          tmem_ld_wait();
+          release(last);
+          if (!more) {
+            add(32, r1, f);
+            break;
+          }
+          ok = ready(tried);
+          if (!ok) break;
+          tmem_ld<32>(tbase + buf * kF8Block, r0);
+          const float f1 = factor();
+          add(32, r1, f);
+          f = f1;
+        }
+      }
+    } else {
+      while (ok) {
+        const float f = factor();
 #pragma unroll
         for (int c = 0; c < kCols; c += kLd) {
           uint32_t r[kLd];
           tmem_ld<kLd>(tbase + buf * kF8Block + c, r);
           tmem_ld_wait();
-          if (c + kLd == kCols) {  // all read: the next but one group may overwrite it
-            tc_fence_before();
-            if (lane == 0) mbar_arrive(&tempty[buf]);
-          }
+          if (c + kLd == kCols) release(buf);
 #pragma unroll
           for (int i = 0; i < kLd; ++i) acc[c + i] = fmaf(__uint_as_float(r[i]), f, acc[c + i]);
         }
-      } else if (lane == 0) {
-        mbar_arrive(&tempty[buf]);
+        advance();
+        if (--groups == 0) break;
+        ok = ready(try_ready());
       }
-      if (++st == stages) { st = 0; phase ^= 1; }
-      buf ^= 1;
     }
     // every group is done: the ring is idle and takes the output, or this split's partial tile
     if (ok && live) {
@@ -490,15 +574,11 @@ __global__ void __launch_bounds__(kF8SmallThreads, 2)
   __syncthreads();
   if (warp == 9) {
     tc_fence_after();
-    f8_tmem_dealloc<false>(tmem, 2 * kF8Block);
+    f8_tmem_dealloc<false>(*reinterpret_cast<volatile uint32_t*>(&bars.tmem_holder), kBufs * kF8Block);
   }
 }
 
 // ------------------------------------------------------------------------------ CTA pairs
-// The scales of one group: of the CTA's 128 tokens and of the tile's two weight blocks.
-struct F8Scales {
-  float x[kF8TileM], w[4];
-};
 constexpr int kF8Slots = kF8PairStages + 2;
 struct F8PairBarriers {
   uint64_t full[kF8PairStages], done[2][kF8PairStages], sfull[kF8Slots], tempty[2][2];
@@ -511,14 +591,38 @@ constexpr size_t kF8PairOut = static_cast<size_t>(kF8EpiWarps) * kF8PairPieces *
 constexpr size_t kF8PairSmem = kF8PairOut + kF8PairStages * 2 * kF8TileBytes + sizeof(F8PairBarriers);
 static_assert(kF8PairSmem <= 227 * 1024, "shared memory of a CTA");
 
+// The tiles of one CTA pair, every (gridDim / 2)-th of the token-major list, without a division per tile.
+struct F8TileWalk {
+  int m, n, m_tiles, n_tiles, dm, dn;
+  SPECB200_DEVINL explicit F8TileWalk(const F8Args& a) : m_tiles(a.m_tiles), n_tiles(a.n_tiles) {
+    const int first = static_cast<int>(blockIdx.x) / 2, step = static_cast<int>(gridDim.x) / 2;
+    m = first % m_tiles;
+    n = first / m_tiles;
+    dm = step % m_tiles;
+    dn = step / m_tiles;
+  }
+  SPECB200_DEVINL bool more() const { return n < n_tiles; }
+  SPECB200_DEVINL void next() {
+    m += dm;
+    n += dn;
+    if (m >= m_tiles) {
+      m -= m_tiles;
+      ++n;
+    }
+  }
+  SPECB200_DEVINL int token0(int rank) const { return (2 * m + rank) * kF8TileM; }
+  SPECB200_DEVINL int feature0() const { return n * 2 * kF8Block; }
+};
+
 // A group's 256 features are multiplied in two halves with a TMEM buffer each (two groups' worth in
 // all): half h holds features 64 h..64 h + 63 of either weight block, so that each epilogue thread reads 64
 // columns of a half. What a buffer costs besides its MMAs -- the commit's and the release's way
 // between warps and CTAs, the read -- then hides behind three other buffers' MMAs; with one buffer per group it
 // did not (8192 x 16384 x 2048: 253 us).
-// Warps 0-7 read back (w on TMEM lane quarter w % 4, weight block w / 4), warp 8 issues TMA, warps 9
-// and 10 of the pair's first CTA tcgen05.mma for both (MMAs issue in order and block the warp while the
-// tensor cores are busy, so two warps take turns), warp 11 fetches scales.
+// Warps 0-7 read back (w on TMEM lane quarter w % 4, weight block w / 4), warps 9
+// and 10 of the pair's first CTA tcgen05.mma for both; warps 8 and 11 load operands and scales. Either
+// kind takes turns: MMAs issue in order and block the warp while the tensor cores are busy, and a
+// load of operands and scales takes its warp longer to issue than the MMAs of a group run.
 __global__ void __launch_bounds__(kF8PairThreads, 1)
     gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map,
                          const __grid_constant__ CUtensorMap y_map, F8Args a) {
@@ -551,70 +655,56 @@ __global__ void __launch_bounds__(kF8PairThreads, 1)
   pdl_launch_dependents();  // as in the small kernel, after the allocation
 
   const int rank = static_cast<int>(cluster_rank());
-  const int first = static_cast<int>(blockIdx.x) / 2, step = static_cast<int>(gridDim.x) / 2;
-  const int tiles = a.m_tiles * a.n_tiles, kblocks = a.kblocks;
-  auto tile_m = [&](int t) { return (t % a.m_tiles * 2 + rank) * kF8TileM; };
-  auto tile_n = [&](int t) { return t / a.m_tiles * 2 * kF8Block; };
+  const int kblocks = a.kblocks;
 
   // 384 threads start with 168 registers each, 64,512; the shares below sum to 7,168 + 57,344.
   if (warp >= kF8EpiWarps) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    if (warp == 8) {
+    if (warp == 8 || warp == 11) {
+      // Every other group each: one lane loads the operands by TMA, all lanes copy the scales, into a
+      // ring of two slots more than there are stages. Once the stage of group g is done, the
+      // epilogue has read the scales of group g - 2 (the MMAs of g waited for that), whose slot and
+      // barrier come next. No barrier can run two phases ahead of a wait for it: the MMAs of a
+      // stage's next group wait for loads that follow the wait for its last one.
       if (lane == 0) {
         tma_prefetch_desc(&w_map);
         tma_prefetch_desc(&x_map);
-        pdl_wait();
-        uint32_t st = 0, phase = 0, issued = 0;
-        bool ok = true;
-        for (int t = first; t < tiles && ok; t += step) {
-          const int m0 = tile_m(t), n0 = tile_n(t) + rank * kF8Block;
-          for (int kb = 0; kb < kblocks; ++kb) {
-            ok = mbar_wait_bounded(&bars.done[1][st], phase ^ 1, a.status, &abort_flag);
-            if (!ok) break;
-            uint8_t* s = ring + st * kStageBytes;
-            if (rank == 0) mbar_arrive_expect_tx(&bars.full[st], 2 * kStageBytes);  // both CTAs' loads
-            const uint32_t bar = cluster_addr(smem_u32(&bars.full[st]), 0);
-            tma_load_2d_pair(s, &w_map, bar, kb * kFp8Group, n0);
-            tma_load_2d_pair(s + kF8TileBytes, &x_map, bar, kb * kFp8Group, m0);
-            if (issued < kF8PairStages) ++issued;
-            if (++st == kF8PairStages) { st = 0; phase ^= 1; }
-          }
-        }
-        // Tail: the last use of every stage is done (so no commit arrives after the exit), or, where
-        // a wait gave up, at least every copy in flight has had its time to land.
-        for (uint32_t i = 0; i < issued; ++i) {
-          if (st == 0) { st = kF8PairStages; phase ^= 1; }
-          --st;
-          if (ok) ok = mbar_wait_bounded(&bars.done[1][st], phase, a.status, &abort_flag);
-          if (!ok) mbar_wait_bounded(rank == 0 ? &bars.full[st] : &bars.done[1][st], phase, a.status, nullptr);
-        }
       }
-    } else if (warp == 11) {
-      // The scales, into a ring of two slots more than there are stages: once the stage of group g
-      // is done, the epilogue has read the scales of group g - 2 (the MMAs of g waited for that),
-      // whose slot and barrier come next.
       pdl_wait();
-      uint32_t st = 0, phase = 0, slot = 0;
-      bool ok = true;
-      for (int t = first; t < tiles && ok; t += step) {
-        const int m0 = tile_m(t) + lane, block = tile_n(t) / kF8Block + lane;
-        const float* sx = a.xs + static_cast<int64_t>(m0) * kblocks;
+      const bool odd = warp == 11;
+      const int64_t pitch = static_cast<int64_t>(32) * kblocks;
+      uint32_t st = 0, phase = 0, slot = 0, last = 0, last_phase = 0;
+      bool ok = true, mine = !odd, any = false;
+      for (F8TileWalk tile(a); tile.more() && ok; tile.next()) {
+        const int m0 = tile.token0(rank), n0 = tile.feature0(), block = 2 * tile.n + lane;
+        const float* sx = a.xs + static_cast<int64_t>(m0 + lane) * kblocks;
         const float* sw = a.ws + static_cast<int64_t>(block) * kblocks;
-        const int64_t pitch = static_cast<int64_t>(32) * kblocks;
         const bool live_w = lane < 2 && block * kF8Block < a.N;
-        for (int kb = 0; kb < kblocks; ++kb) {
-          ok = wait_warp(&bars.done[1][st], phase ^ 1, a.status, &abort_flag);
-          if (!ok) break;
-          F8Scales& to = bars.scales[slot];
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (m0 + 32 * i < a.M) copy_async_4(&to.x[32 * i + lane], sx + i * pitch + kb);
-          if (live_w) copy_async_4(&to.w[lane], sw + kb);
-          copy_async_arrive(&bars.sfull[slot]);
+        for (int kb = 0; kb < kblocks; ++kb, mine = !mine) {
+          if (mine) {
+            ok = wait_warp(&bars.done[1][st], phase ^ 1, a.status, &abort_flag);
+            if (!ok) break;
+            if (lane == 0) {
+              uint8_t* s = ring + st * kStageBytes;
+              if (rank == 0) mbar_arrive_expect_tx(&bars.full[st], 2 * kStageBytes);  // both CTAs' loads
+              const uint32_t bar = cluster_addr(smem_u32(&bars.full[st]), 0);
+              tma_load_2d_pair(s, &w_map, bar, kb * kFp8Group, n0 + rank * kF8Block);
+              tma_load_2d_pair(s + kF8TileBytes, &x_map, bar, kb * kFp8Group, m0);
+            }
+            __syncwarp();
+            copy_scales(bars.scales[slot], &bars.sfull[slot], sx + kb, sw + kb, pitch, a.M - m0, live_w, lane);
+            any = true;
+            last = st;
+            last_phase = phase;
+          }
           if (++st == kF8PairStages) { st = 0; phase ^= 1; }
           if (++slot == kF8Slots) slot = 0;
         }
       }
+      // Tail: this warp's last group is done, and with it all earlier ones (so no commit arrives after
+      // the exit), or, where a wait gave up, its copies in flight have had their time to land.
+      if (any && ok) ok = wait_warp(&bars.done[1][last], last_phase, a.status, &abort_flag);
+      if (any && !ok && lane == 0) mbar_wait_bounded(rank == 0 ? &bars.full[last] : &bars.done[1][last], last_phase, a.status, nullptr);
       asm volatile("cp.async.wait_all;" ::: "memory");
     } else if (rank == 0) {  // warps 9 and 10: every other group each
       constexpr uint32_t idesc = umma_idesc_e4m3(2 * kF8TileM, kF8Block);
@@ -623,7 +713,7 @@ __global__ void __launch_bounds__(kF8PairThreads, 1)
       const uint32_t turn = static_cast<uint32_t>(warp - 9);
       uint32_t st = 0, phase = 0, buf = 0, acc_phase = 0;
       bool ok = true;
-      for (int t = first; t < tiles && ok; t += step) {
+      for (F8TileWalk tile(a); tile.more() && ok; tile.next()) {
         for (int kb = 0; kb < kblocks; ++kb) {
           if (buf == turn) {
             const uint64_t at = static_cast<uint64_t>(st * (kStageBytes >> 4));
@@ -674,8 +764,8 @@ __global__ void __launch_bounds__(kF8PairThreads, 1)
       return __all_sync(0xffffffffu, tried) || wait_warp(&bars.done[1][st], phase, a.status, &abort_flag);
     };
     auto factor = [&] { return bars.scales[slot].x[quarter * 32 + lane] * bars.scales[slot].w[block]; };
-    for (int t = first; t < tiles && ok; t += step) {
-      const int m0 = tile_m(t) + quarter * 32, n0 = tile_n(t) + block * kF8Block;
+    for (F8TileWalk tile(a); tile.more() && ok; tile.next()) {
+      const int m0 = tile.token0(rank) + quarter * 32, n0 = tile.feature0() + block * kF8Block;
       if (m0 >= a.M || n0 >= a.N) {  // a warp without outputs only keeps step
         for (int kb = 0; kb < kblocks; ++kb) {
           ok = first_ready(false) && second_ready(false);
@@ -686,56 +776,54 @@ __global__ void __launch_bounds__(kF8PairThreads, 1)
         }
         continue;
       }
-      float acc[kCols];
+      f32x2 acc2[kCols / 2];
 #pragma unroll
-      for (int i = 0; i < kCols; ++i) acc[i] = 0.f;
+      for (int i = 0; i < kCols / 2; ++i) acc2[i] = 0;
       // 32 columns come back at a time, the next ones and the next poll on their way while the last
       // ones are added.
       uint32_t r0[kLd], r1[kLd];
       auto add = [&](int c, const uint32_t (&r)[kLd], float f) {
 #pragma unroll
-        for (int i = 0; i < kLd; ++i) acc[c + i] = fmaf(__uint_as_float(r[i]), f, acc[c + i]);
+        for (int i = 0; i < kLd; i += 2) add2(acc2[(c + i) / 2], r[i], r[i + 1], f);
       };
       ok = first_ready(try_first());
       if (!ok) break;
       tc_fence_after();
       float f = factor();
       tmem_ld<kLd>(tbase + buf * 256, r0);
+      tmem_ld<kLd>(tbase + buf * 256 + 32, r1);
       for (int kb = 0;;) {
         const uint32_t at = tbase + buf * 256;
         tmem_ld_wait();
-        tmem_ld<kLd>(at + 32, r1);
+        release(0);
         const bool second = try_second();
         add(0, r0, f);
-        tmem_ld_wait();
-        release(0);
+        add(32, r1, f);
         ok = second_ready(second);
         if (!ok) break;
         tc_fence_after();
         tmem_ld<kLd>(at + 128, r0);
-        add(32, r1, f);
-        tmem_ld_wait();
         tmem_ld<kLd>(at + 160, r1);
+        tmem_ld_wait();
         const uint32_t last = buf;
         next_group();
-        const bool more = ++kb < kblocks, next = more && try_first();
-        add(64, r0, f);
-        tmem_ld_wait();
         tc_fence_before();
         mbar_arrive_cluster_if(lane == 0, tempty0 + (last * 2 + 1) * sizeof(uint64_t));
-        if (!more) {
-          add(96, r1, f);
-          break;
-        }
+        const bool more = ++kb < kblocks, next = more && try_first();
+        add(64, r0, f);
+        add(96, r1, f);
+        if (!more) break;
         ok = first_ready(next);
         if (!ok) break;
         tc_fence_after();
         tmem_ld<kLd>(tbase + buf * 256, r0);
-        const float f1 = factor();
-        add(96, r1, f);
-        f = f1;
+        tmem_ld<kLd>(tbase + buf * 256 + 32, r1);
+        f = factor();
       }
       if (!ok) break;
+      float acc[kCols];
+#pragma unroll
+      for (int i = 0; i < kCols / 2; ++i) asm("mov.b64 {%0, %1}, %2;" : "=f"(acc[2 * i]), "=f"(acc[2 * i + 1]) : "l"(acc2[i]));
       if (a.out_f32)
         store_warp_tile<float, kF8PairPieces>(a, y_map, acc, out_buf, m0, n0, lane);
       else
@@ -756,6 +844,7 @@ __global__ void __launch_bounds__(kF8PairThreads, 1)
 // ------------------------------------------------------------------------------ host side
 struct F8Plan {
   bool pair;
+  int per_sm;  // CTAs per SM that the small kernel is cut for
   int splits, stages, box_rows;
   int kblocks, m_tiles, n_tiles;
   size_t ring, smem;
@@ -778,17 +867,21 @@ F8Plan plan_fp8(int M, int N, int K) {
   p.m_tiles = (M + kF8TileM - 1) / kF8TileM;
   p.n_tiles = (N + kF8Block - 1) / kF8Block;
   const int64_t tiles = static_cast<int64_t>(p.m_tiles) * p.n_tiles;
+  const char* fs = getenv("F8_SPLITS"); const char* fp = getenv("F8_PERSM");
   while (p.splits < kF8MaxSplits && tiles * p.splits * 2 <= 2 * 148 && p.kblocks >= 4 * p.splits) p.splits *= 2;
+  if (fs) p.splits = std::min(atoi(fs), p.kblocks);
+  p.per_sm = tiles * p.splits <= 148 ? 1 : 2;
+  if (fp) p.per_sm = atoi(fp);
   const size_t x_bytes = static_cast<size_t>(p.box_rows) * kFp8Group, stage = kF8TileBytes + x_bytes;
   // An MMA reads 128 token rows: with fewer in a box it runs on into the next stage, whose lanes
   // are never read back; the last stage needs that much room behind it.
   const size_t slack = kF8TileBytes - x_bytes;
   // 228 KB per SM, of which each CTA takes 1 KB for itself: 113 KB each for two CTAs
-  const size_t budget = 113 * 1024 - sizeof(F8SmallBarriers);
-  p.stages = static_cast<int>(std::min<size_t>(kF8MaxStages, (budget - slack) / stage));
+  const size_t fixed = sizeof(F8SmallBarriers) + 4 * sizeof(F8Scales);
+  p.stages = static_cast<int>(std::min<size_t>(kF8MaxStages, ((p.per_sm == 1 ? 227 : 113) * 1024 - fixed - slack) / (stage + sizeof(F8Scales))));
   p.ring = std::max(p.stages * stage + slack, p.splits > 1 ? static_cast<size_t>(p.box_rows) * (kF8Block + 4) * 4
                                                            : static_cast<size_t>(kF8EpiWarps) * kF8OutPiece);
-  p.smem = p.ring + sizeof(F8SmallBarriers);
+  p.smem = fixed + p.ring + p.stages * sizeof(F8Scales);
   return p;
 }
 
@@ -807,8 +900,10 @@ cudaError_t prepare_fp8(K kernel, std::atomic<bool> (&ready)[kF8MaxDevices]) {
 
 cudaError_t launch_fp8(const F8Plan& p, const CUtensorMap& wm, const CUtensorMap& xm, const CUtensorMap& ym, const F8Args& a,
                        cudaStream_t s) {
-  static std::atomic<bool> small_ready[kF8MaxDevices], pair_ready[kF8MaxDevices];
-  const cudaError_t e = p.pair ? prepare_fp8(gemm_fp8_pair_kernel, pair_ready) : prepare_fp8(gemm_fp8_small_kernel, small_ready);
+  static std::atomic<bool> ready[3][kF8MaxDevices];
+  const cudaError_t e = p.pair          ? prepare_fp8(gemm_fp8_pair_kernel, ready[0])
+                        : p.per_sm == 1 ? prepare_fp8(gemm_fp8_small_kernel<1>, ready[1])
+                                        : prepare_fp8(gemm_fp8_small_kernel<2>, ready[2]);
   if (e != cudaSuccess) return e;
   const int64_t tiles = static_cast<int64_t>(p.m_tiles) * p.n_tiles;
   const int cluster = p.pair ? 2 : p.splits;
@@ -827,7 +922,8 @@ cudaError_t launch_fp8(const F8Plan& p, const CUtensorMap& wm, const CUtensorMap
   cfg.attrs = attr;
   cfg.numAttrs = cluster > 1 ? 2 : 1;
   return p.pair ? cudaLaunchKernelEx(&cfg, gemm_fp8_pair_kernel, wm, xm, ym, a)
-                : cudaLaunchKernelEx(&cfg, gemm_fp8_small_kernel, wm, xm, ym, a);
+                : p.per_sm == 1 ? cudaLaunchKernelEx(&cfg, gemm_fp8_small_kernel<1>, wm, xm, ym, a)
+                                : cudaLaunchKernelEx(&cfg, gemm_fp8_small_kernel<2>, wm, xm, ym, a);
 }
 
 }  // namespace
