@@ -18,7 +18,6 @@
 //   instead of 48, and holds 128 tokens of the accumulators.
 #include <algorithm>
 #include <atomic>
-#include <cstdlib>
 
 #include "fp8.cuh"
 #include "gemm.cuh"
@@ -28,11 +27,14 @@ namespace {
 
 constexpr int kF8TileM = 128;
 constexpr int kF8Block = 128;     // features per weight block
-constexpr int kF8MaxSplits = 8;
+constexpr int kF8MaxSplits = 4;
 constexpr int kF8MaxStages = 12;
 constexpr int kF8MaxDevices = 64;
 constexpr int kF8EpiWarps = 8;
-constexpr int kF8SmallThreads = 320;
+// The small kernel is cut for one or two CTAs per SM: alone a CTA has four TMEM buffers, twice the
+// ring, a second producer warp and registers to read ahead.
+__host__ __device__ constexpr int f8_small_threads(int per_sm) { return per_sm == 1 ? 352 : 320; }
+__host__ __device__ constexpr int f8_small_bufs(int per_sm) { return per_sm == 1 ? 4 : 2; }
 constexpr int kF8PairThreads = 384;
 constexpr int kF8PairStages = 4;
 constexpr int kF8OutPiece = 4096; // 32 rows x 128 bytes of output on their way to memory
@@ -49,6 +51,7 @@ struct F8Args {
   int64_t ldy;
   int out_f32;
   int rows16;           // y's rows are on 16-byte boundaries: tiles are written by TMA, split ones in quads
+  int tail16;           // ... and end on one
   int32_t* status;
 };
 
@@ -258,8 +261,8 @@ SPECB200_DEVINL void tma_store_2d(const CUtensorMap* map, const void* smem_src, 
 // One warp's 32 tokens x kCols features to memory through kPieces pieces of shared memory, a piece
 // being 128 bytes per row (64 bf16 or 32 fp32 features). The 16-byte units of a row are swizzled by
 // the row (the 128-byte swizzle TMA reads), so that neither side has bank conflicts. TMA stores
-// leave the warp free while the pieces drain; an output whose rows are off the 16-byte boundaries is
-// written by the warp itself.
+// leave the warp free while the pieces drain; what lies off the 16-byte boundaries is written by the
+// warp itself.
 template <typename T, int kPieces, int kCols>
 SPECB200_DEVINL void store_warp_tile(const F8Args& a, const CUtensorMap& y_map, const float (&acc)[kCols],
                                      uint8_t* bufs, int m0, int n0, int lane) {
@@ -287,19 +290,18 @@ SPECB200_DEVINL void store_warp_tile(const F8Args& a, const CUtensorMap& y_map, 
       *reinterpret_cast<uint4*>(bufs + piece * kF8OutPiece + lane * 128 + ((unit ^ lane) & 7) * 16) =
           make_uint4(v[0], v[1], v[2], v[3]);
     }
-    if (a.rows16) {
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) {
-#pragma unroll
-        for (int c = c0; c < c0 + kRound; c += kPiece)
-          if (n0 + c < a.N) tma_store_2d(&y_map, bufs + (c - c0) / kPiece * kF8OutPiece, n0 + c, m0);
-        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-      }
-      continue;
-    }
+    // a piece that the row's end cuts off its 16-byte grid is not TMA's: it would fill the last unit
+    auto by_tma = [&](int c) { return a.rows16 && (a.tail16 || n0 + c + kPiece <= a.N); };
+    if (a.rows16) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncwarp();
+    if (a.rows16 && lane == 0) {
+#pragma unroll
+      for (int c = c0; c < c0 + kRound; c += kPiece)
+        if (n0 + c < a.N && by_tma(c)) tma_store_2d(&y_map, bufs + (c - c0) / kPiece * kF8OutPiece, n0 + c, m0);
+      asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+    }
     for (int c = c0; c < c0 + kRound; c += kPiece) {
+      if (by_tma(c)) continue;
       const int n = n0 + c + (lane & 7) * kUnit;
       for (int r = lane >> 3; r < 32; r += 4) {
         const uint4 q = *reinterpret_cast<const uint4*>(bufs + (c - c0) / kPiece * kF8OutPiece + r * 128 + ((lane ^ r) & 7) * 16);
@@ -336,16 +338,17 @@ SPECB200_DEVINL void copy_scales(F8Scales& to, uint64_t* filled, const float* sx
   copy_async_arrive(filled);
 }
 
-// Warps 0-7 read back (w on TMEM lane quarter w % 4, columns 64 (w / 4)..), warp 8 issues TMA and
-// fetches scales, warp 9 tcgen05.mma. A stage's `done` barrier frees its operands and completes its
+// Warps 0-7 read back (w on TMEM lane quarter w % 4, columns 64 (w / 4)..), warp 8 (and 10) loads
+// operands and scales, warp 9 issues tcgen05.mma. A stage's `done` barrier frees its operands and completes its
 // accumulator. Small calls are bound by latency, so loads start before TMEM is allocated: the
 // epilogue learns of the allocation through the first `done`.
 template <int kPerSm>
-__global__ void __launch_bounds__(kF8SmallThreads, kPerSm)
+__global__ void __launch_bounds__(f8_small_threads(kPerSm), kPerSm)
     gemm_fp8_small_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map,
                           const __grid_constant__ CUtensorMap y_map, F8Args a) {
   constexpr int kCols = 64;                  // features per epilogue thread
-  constexpr int kBufs = kPerSm == 1 ? 4 : 2; // TMEM buffers
+  constexpr int kThreads = f8_small_threads(kPerSm), kBufs = f8_small_bufs(kPerSm);
+  constexpr int kProducers = kPerSm == 1 ? 2 : 1;
   constexpr int kLd = kPerSm == 1 ? 32 : 16; // accumulator columns read back at a time (what registers allow)
   constexpr int kPitch = kF8Block + 4;       // partial tile's row pitch (floats)
   // the ring (1024-byte swizzle atoms), which ends up holding the output; barriers; scales
@@ -379,12 +382,14 @@ __global__ void __launch_bounds__(kF8SmallThreads, kPerSm)
   const int kb0 = static_cast<int>(static_cast<int64_t>(a.kblocks) * split / splits);
   const int kb1 = static_cast<int>(static_cast<int64_t>(a.kblocks) * (split + 1) / splits);
 
-  if (warp == 8) {
+  if (warp == 8 || warp == 10) {
+    // One lane loads a group's operands by TMA, all lanes copy its scales; two producers take turns
+    // (one takes about 700 cycles per group to issue it all).
     pdl_wait();
     const float* sx = a.xs + static_cast<int64_t>(tile_m + lane) * a.kblocks + kb0;
     const float* sw = a.ws + static_cast<int64_t>(tile_n / kF8Block) * a.kblocks + kb0;
     const int64_t pitch32 = static_cast<int64_t>(32) * a.kblocks;
-    const int tokens = a.M - tile_m, groups = kb1 - kb0;
+    const int tokens = a.M - tile_m, groups = kb1 - kb0, me = warp == 8 ? 0 : 1;
     auto load = [&](int g, uint32_t st) {
       if (lane == 0) {
         uint8_t* s = smem + st * stage_bytes;
@@ -392,39 +397,42 @@ __global__ void __launch_bounds__(kF8SmallThreads, kPerSm)
         tma_load_2d(s, &w_map, &full[st], (kb0 + g) * kFp8Group, tile_n);
         tma_load_2d(s + kF8TileBytes, &x_map, &full[st], (kb0 + g) * kFp8Group, tile_m);
       }
+      __syncwarp();
     };
     auto fetch = [&](int g, uint32_t slot) {
       copy_scales(scales[slot], &sfull[slot], sx + g, sw + g, pitch32, tokens, lane == 0, lane);
     };
-    // The ring's first filling waits for nothing: operands first, then their scales. A slot of
-    // scales is used again kBufs groups later than a stage (see gemm_fp8_pair_kernel).
+    // The ring's first filling waits for nothing: operands first, then their scales. Scales have
+    // kBufs slots more than there are stages: when a stage is done, so are the MMAs that waited for
+    // the epilogue to read the slot that comes next. No barrier can run two phases ahead of a wait for
+    // it, as there are at least kBufs stages.
     const int first = min(groups, static_cast<int>(stages));
-    for (int g = 0; g < first; ++g) load(g, g);
-    for (int g = 0; g < first; ++g) fetch(g, g);
+    for (int g = me; g < first; g += kProducers) load(g, g);
+    for (int g = me; g < first; g += kProducers) fetch(g, g);
     uint32_t st = 0, phase = 0, slot = stages;
-    bool ok = true;
     for (int g = first; g < groups; ++g) {
-      ok = wait_warp(&done[st], phase, a.status, &abort_flag);
-      if (!ok) break;
-      load(g, st);
-      fetch(g, slot);
+      if (kProducers == 1 || g % kProducers == me) {
+        if (!wait_warp(&done[st], phase, a.status, &abort_flag)) {
+          // gave up: this warp's copies in flight get their time to land
+          for (int i = max(0, g - static_cast<int>(stages)); i < g; ++i)
+            if (lane == 0 && i % kProducers == me)
+              mbar_wait_bounded(&full[i % stages], (i / stages) & 1, a.status, nullptr);
+          break;
+        }
+        load(g, st);
+        fetch(g, slot);
+      }
       if (++st == stages) { st = 0; phase ^= 1; }
       if (++slot == stages + kBufs) slot = 0;
     }
-    // Tail: the last use of every stage is done (so no commit arrives after the exit), or, where a
-    // wait gave up, at least every copy in flight has landed.
-    for (int i = 0; i < first; ++i) {
-      const uint32_t s = first < static_cast<int>(stages) ? i : st, p = phase;
-      if (++st == stages) { st = 0; phase ^= 1; }
-      if (ok) ok = wait_warp(&done[s], p, a.status, &abort_flag);
-      if (!ok && lane == 0) mbar_wait_bounded(&full[s], p, a.status, nullptr);
-      __syncwarp();
-    }
+    __syncwarp();
     asm volatile("cp.async.wait_all;" ::: "memory");
     pdl_launch_dependents();
   } else if (warp == 9) {
     f8_tmem_alloc<false>(&bars.tmem_holder, kBufs * kF8Block);
+    tc_fence_before();
     __syncwarp();
+    tc_fence_after();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&bars.tmem_holder);
     // Only from here on may the next kernel's CTAs start (each warp allows it once it knows of the
     // allocation): one that allocated TMEM before this CTA and then waited for it would keep it
@@ -482,7 +490,7 @@ __global__ void __launch_bounds__(kF8SmallThreads, kPerSm)
       }
     } else if constexpr (kPerSm == 1) {
       // 32 columns come back at a time, the next ones and the next group's poll on their way while
-      // the last ones are added: 
+      // the last ones are added.
       uint32_t r0[32], r1[32];
       auto add = [&](int c, const uint32_t (&r)[32], float f) {
 #pragma unroll
@@ -552,19 +560,17 @@ __global__ void __launch_bounds__(kF8SmallThreads, kPerSm)
     constexpr int kQuads = kF8Block / 4;
     if (!*reinterpret_cast<volatile int*>(&abort_flag)) {
       const uint32_t base = smem_u32(smem);
-      for (int i = split * kF8SmallThreads + threadIdx.x; i < rows * kQuads; i += splits * kF8SmallThreads) {
+      for (int i = split * kThreads + threadIdx.x; i < rows * kQuads; i += splits * kThreads) {
         const int r = i / kQuads, c = (i % kQuads) * 4;
         if (tile_n + c >= a.N) continue;
         float v[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int p0 = 0; p0 < splits; p0 += 4) {  // four splits' loads in flight, added in split order
-          float4 q[4];
+        float4 q[kF8MaxSplits];  // all splits' loads in flight, added in split order
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (p0 + j < splits) q[j] = ld_cluster_f4(base + (r * kPitch + c) * 4, p0 + j);
+        for (int p = 0; p < kF8MaxSplits; ++p)
+          if (p < splits) q[p] = ld_cluster_f4(base + (r * kPitch + c) * 4, p);
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (p0 + j < splits) { v[0] += q[j].x; v[1] += q[j].y; v[2] += q[j].z; v[3] += q[j].w; }
-        }
+        for (int p = 0; p < kF8MaxSplits; ++p)
+          if (p < splits) { v[0] += q[p].x; v[1] += q[p].y; v[2] += q[p].z; v[3] += q[p].w; }
         store_quad(a, static_cast<int64_t>(tile_m + r) * a.ldy + tile_n + c, a.N - tile_n - c, v);
       }
     }
@@ -853,31 +859,36 @@ struct F8Plan {
 F8Plan plan_fp8(int M, int N, int K) {
   F8Plan p = {};
   p.kblocks = (K + kFp8Group - 1) / kFp8Group;
-  const int pair_m = (M + 2 * kF8TileM - 1) / (2 * kF8TileM), pair_n = (N + 2 * kF8Block - 1) / (2 * kF8Block);
-  p.pair = M > kF8TileM && static_cast<int64_t>(pair_m) * pair_n >= 148;
-  p.splits = 1;
   p.box_rows = std::min(kF8TileM, (M + 7) / 8 * 8);
+  p.m_tiles = (M + kF8TileM - 1) / kF8TileM;
+  p.n_tiles = (N + kF8Block - 1) / kF8Block;
+  p.splits = 1;
+  const int64_t tiles = static_cast<int64_t>(p.m_tiles) * p.n_tiles;
+  // More than one tile per SM and tokens for pairs: pairs, although their last wave may be partial
+  // (512 x 16384 x 2048: 21.1 us against 25.4 on small tiles; 160 x 16384 x 2048: 13.1 against 12.7).
+  p.pair = M > kF8TileM && tiles > 148;
   if (p.pair) {
-    p.m_tiles = pair_m;
-    p.n_tiles = pair_n;
+    p.m_tiles = (p.m_tiles + 1) / 2;
+    p.n_tiles = (p.n_tiles + 1) / 2;
     p.stages = kF8PairStages;
     p.smem = kF8PairSmem;
     return p;
   }
-  p.m_tiles = (M + kF8TileM - 1) / kF8TileM;
-  p.n_tiles = (N + kF8Block - 1) / kF8Block;
-  const int64_t tiles = static_cast<int64_t>(p.m_tiles) * p.n_tiles;
-  const char* fs = getenv("F8_SPLITS"); const char* fp = getenv("F8_PERSM");
-  while (p.splits < kF8MaxSplits && tiles * p.splits * 2 <= 2 * 148 && p.kblocks >= 4 * p.splits) p.splits *= 2;
-  if (fs) p.splits = std::min(atoi(fs), p.kblocks);
-  p.per_sm = tiles * p.splits <= 148 ? 1 : 2;
-  if (fp) p.per_sm = atoi(fp);
+  // A group takes a CTA alone on its SM about 0.29 us, and the exchange of partial tiles 1.4-2.5 us
+  // (more for more tokens): K is split where it is long enough to win that back, at most four
+  // ways, and only while all clusters find room at once (four CTAs of an SM each do not fill every
+  // GPC). Decode 1 x 6144 x 2048: 6.9 us unsplit, 6.5 split in two; 320 x 2048 x 8192: 22.1 and 15.5;
+  // 320 x 2048 x 2048: 7.5 and 8.0.
+  p.per_sm = tiles <= 148 ? 1 : 2;
+  if (p.kblocks >= (p.box_rows <= 32 ? 16 : 24))
+    while (p.splits < kF8MaxSplits && tiles * p.splits * 2 <= (p.splits == 1 ? 148 : 128) && p.kblocks >= 8 * p.splits)
+      p.splits *= 2;
   const size_t x_bytes = static_cast<size_t>(p.box_rows) * kFp8Group, stage = kF8TileBytes + x_bytes;
   // An MMA reads 128 token rows: with fewer in a box it runs on into the next stage, whose lanes
   // are never read back; the last stage needs that much room behind it.
   const size_t slack = kF8TileBytes - x_bytes;
   // 228 KB per SM, of which each CTA takes 1 KB for itself: 113 KB each for two CTAs
-  const size_t fixed = sizeof(F8SmallBarriers) + 4 * sizeof(F8Scales);
+  const size_t fixed = sizeof(F8SmallBarriers) + f8_small_bufs(p.per_sm) * sizeof(F8Scales);
   p.stages = static_cast<int>(std::min<size_t>(kF8MaxStages, ((p.per_sm == 1 ? 227 : 113) * 1024 - fixed - slack) / (stage + sizeof(F8Scales))));
   p.ring = std::max(p.stages * stage + slack, p.splits > 1 ? static_cast<size_t>(p.box_rows) * (kF8Block + 4) * 4
                                                            : static_cast<size_t>(kF8EpiWarps) * kF8OutPiece);
@@ -909,7 +920,7 @@ cudaError_t launch_fp8(const F8Plan& p, const CUtensorMap& wm, const CUtensorMap
   const int cluster = p.pair ? 2 : p.splits;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>((p.pair ? std::min<int64_t>(tiles, 74) : tiles) * cluster));
-  cfg.blockDim = dim3(p.pair ? kF8PairThreads : kF8SmallThreads);
+  cfg.blockDim = dim3(p.pair ? kF8PairThreads : f8_small_threads(p.per_sm));
   cfg.dynamicSmemBytes = p.smem;
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
@@ -975,6 +986,7 @@ extern "C" int specb200_linear_fp8(const void* x, int64_t ldx, const float* x_sc
   a.ldy = ldy;
   a.out_f32 = out_f32 ? 1 : 0;
   a.rows16 = y_rows16;
+  a.tail16 = (static_cast<int64_t>(N) * esize) % 16 == 0;
   a.status = status;
   cudaError_t e = cudaSuccess;
   if (status) e = cudaMemsetAsync(status, 0, sizeof(int32_t), s);

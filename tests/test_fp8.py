@@ -502,7 +502,8 @@ def test_linear_of_views():
 def test_linear_output_pitch_and_frame():
     """Through the C ABI: an output with a pitch of its own (odd: scalar stores) keeps what lies around it."""
     lib = _lib()
-    for m, n, k, pitch in ((5, 200, 256, 207), (130, 96, 128, 104), (40, 333, 2048, 340)):
+    for m, n, k, pitch in ((5, 200, 256, 207), (130, 96, 128, 104), (40, 333, 2048, 340), (40, 333, 2048, 344),
+                           (3, 77, 4096, 80), (300, 8002, 128, 8008), (300, 8001, 130, 8003)):
         x, xs, w, ws = _operands(m, m, n, k)
         for f32 in (0, 1):
             y = torch.full((m + 2, pitch), 9.0, dtype=F32 if f32 else BF16, device=DEV)
