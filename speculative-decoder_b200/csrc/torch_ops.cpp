@@ -6,6 +6,7 @@
 // specb200/_ffi.py: ValueError for bad arguments, NotImplementedError for types and sizes the
 // kernels do not handle, RuntimeError for tensors that are not on a CUDA device and for CUDA errors.
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -64,6 +65,11 @@ int as_int(const char* where, int64_t v) {
 int64_t groups_of(int64_t k) { return (k + kGroup - 1) / kGroup; }
 int64_t padded(int64_t k) { return (k + 15) / 16 * 16; }
 
+// torch.empty on x's device without the dispatcher (0.25 us of host time less per tensor).
+at::Tensor empty_beside(const at::Tensor& x, at::IntArrayRef sizes, at::ScalarType type) {
+  return at::Tensor(at::detail::empty_cuda(sizes, type, x.device(), std::nullopt));
+}
+
 // [..., K] as M rows of K consecutive elements, `pitch` elements apart (any pitch that fits a
 // single row); copied only if the tensor does not lie like that.
 struct Rows {
@@ -106,12 +112,11 @@ Quantized quantized_like(const at::Tensor& x, int64_t k, at::IntArrayRef scale_s
   Quantized out;
   out.pitch = padded(k);
   c10::SmallVector<int64_t, 6> sizes(x.sizes().begin(), x.sizes().end());
-  const auto device = x.options().requires_grad(false);
   sizes.back() = out.pitch;
-  out.q = at::empty(sizes, device.dtype(at::kFloat8_e4m3fn));
+  out.q = empty_beside(x, sizes, at::kFloat8_e4m3fn);
   if (out.pitch != k) out.q = out.q.narrow(-1, 0, k);
   sizes.back() = groups_of(k);
-  out.scales = at::empty(scale_sizes.empty() ? at::IntArrayRef(sizes) : scale_sizes, device.dtype(at::kFloat));
+  out.scales = empty_beside(x, scale_sizes.empty() ? at::IntArrayRef(sizes) : scale_sizes, at::kFloat);
   return out;
 }
 
@@ -181,7 +186,7 @@ PyObject* rmsnorm(PyObject* const* args) {
   at::Tensor h;
   if (delta) {
     d = rows_of(where, *delta);
-    h = at::empty(x.sizes(), x.options().requires_grad(false));
+    h = empty_beside(x, x.sizes(), x.scalar_type());
   }
   const Here here(x);
   check_rc(where, specb200_rmsnorm_fp8(code, r.ptr, r.pitch, d.ptr, d.pitch, w.data_ptr(), as_int(where, r.m),
@@ -213,7 +218,7 @@ Rows operand_of(const at::Tensor& x, const char* what) {
   if (x.scalar_type() != at::kFloat8_e4m3fn) bad(text(where, ": ", what, " is ", x.scalar_type(), ", not Float8_e4m3fn"));
   Rows r = rows_of(where, x);
   if (r.pitch % 16 || reinterpret_cast<uintptr_t>(r.ptr) % 16) {
-    const at::Tensor bytes = at::empty({r.m, padded(r.k)}, x.options().dtype(at::kByte));
+    const at::Tensor bytes = empty_beside(x, {r.m, padded(r.k)}, at::kByte);
     bytes.narrow(1, 0, r.k).copy_(r.held.detach().reshape({r.m, r.k}).view(at::kByte));
     r.held = bytes;
     r.ptr = bytes.data_ptr();
@@ -245,10 +250,9 @@ PyObject* linear(PyObject* const* args) {
   const at::Tensor ws = w_scales.is_contiguous() ? w_scales : w_scales.detach().contiguous();
   c10::SmallVector<int64_t, 6> sizes(x.sizes().begin(), x.sizes().end());
   sizes.back() = n;
-  const auto device = x.options().requires_grad(false);
-  const at::Tensor y = at::empty(sizes, device.dtype(out_f32 ? at::kFloat : at::kBFloat16));
+  const at::Tensor y = empty_beside(x, sizes, out_f32 ? at::kFloat : at::kBFloat16);
   at::Tensor status;
-  if (check) status = at::empty({1}, device.dtype(at::kInt));
+  if (check) status = empty_beside(x, {1}, at::kInt);
   {
     const Here here(x);
     check_rc(where, specb200_linear_fp8(rx.ptr, rx.pitch, static_cast<const float*>(xs.data_ptr()), rw.ptr, rw.pitch,

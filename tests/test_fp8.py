@@ -544,11 +544,73 @@ def test_linear_is_the_same_every_time_and_in_any_batch():
     assert torch.equal(ops.linear_fp8(x[2:5], xs[2:5], w, ws), y[2:5])
 
 
+# one shape for each way a product is split over CTAs: one tile per SM, K split in two and four, two
+# tiles per SM, pairs with a partial last wave, pairs with an odd number of groups
+PLANS = [(40, 900, 512), (300, 2048, 4096), (3, 2048, 2048), (128, 25600, 256), (700, 12000, 256), (2000, 5000, 384)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", PLANS)
+def test_linear_repeats_bit_for_bit(m, n, k):
+    """Back to back without a wait in between, so that each call starts while the last one ends."""
+    ops = _ops()
+    x, xs, w, ws = _operands(m + n, m, n, k)
+    first = ops.linear_fp8(x, xs, w, ws, out_f32=True)
+    _check_product(first, x, xs, w, ws, True)
+    again = [ops.linear_fp8(x, xs, w, ws, out_f32=True, check=False) for _ in range(30)]
+    assert all(torch.equal(y, first) for y in again)
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits():
+    """More than 2^31 elements in the inputs and the outputs; the last rows are compared."""
+    ops = _ops()
+    m, k, tail = 70_000, 32_768, 40
+    x = torch.zeros(m, k, dtype=BF16, device=DEV)
+    x[-tail:] = _rand(80, tail, k, dtype=BF16)
+    q, s = ops.quantize_fp8(x)
+    _check_quantized(q[-tail:], s[-tail:], x[-tail:].double(), d=4 * U, s_tol=2 * U)
+    del q, s
+    weight = torch.ones(k, dtype=BF16, device=DEV)
+    q, s, h = ops.rmsnorm_fp8(x, weight, 1e-5, delta=x)
+    assert torch.equal(h[-tail:], x[-tail:] + x[-tail:])
+    _check_quantized(q[-tail:], s[-tail:], _norm64(h[-tail:], weight, 1e-5), d=4 * U, s_tol=NORM_S)
+    del q, s, h
+    q, s = ops.silu_mul_fp8(x)
+    g, u = x[-tail:, : k // 2].double(), x[-tail:, k // 2:].double()
+    _check_quantized(q[-tail:], s[-tail:], g * torch.sigmoid(g) * u, **_silu_tol(g))
+    del q, s, x
+    xq, xs, w, ws = _operands(81, m, k, 48)
+    y = ops.linear_fp8(xq, xs, w, ws)
+    _check_product(y[-tail:], xq[-tail:], xs[-tail:], w, ws, False)
+
+
+@pytest.mark.gpu
+def test_capture_with_a_status_word():
+    """Through the C ABI, whose call clears the status word in front of the kernel."""
+    lib = _lib()
+    x, xs, w, ws = _operands(82, 9, 640, 512)
+    y, status = torch.zeros(9, 640, dtype=BF16, device=DEV), torch.full((1,), 5, dtype=torch.int32, device=DEV)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for _ in range(3):
+            rc = lib.specb200_linear_fp8(x.data_ptr(), x.stride(0), xs.data_ptr(), w.data_ptr(), w.stride(0), ws.data_ptr(),
+                                         9, 640, 512, 0, y.data_ptr(), 640, status.data_ptr(),
+                                         torch.cuda.current_stream().cuda_stream)
+            assert rc == 0
+    for _ in range(2):
+        y.zero_()
+        status.fill_(5)
+        graph.replay()
+        assert int(status) == 0
+        _check_product(y, x, xs, w, ws, False)
+
+
 @pytest.mark.gpu
 def test_streams_and_graphs_do_not_share_state():
     """Two streams that overlap, and two captured graphs replayed at once, give each call's own results."""
     ops = _ops()
-    cases = [_operands(50 + i, m, n, k) for i, (m, n, k) in enumerate([(5, 2048, 8192), (40, 2048, 4096)])]
+    cases = [_operands(50 + i, m, n, k) for i, (m, n, k) in enumerate([(5, 2048, 8192), (700, 12000, 256)])]
     want = [ops.linear_fp8(*c) for c in cases]
     acts = [_rand(60 + i, 50, 2048, dtype=BF16) for i in range(2)]
     weight = torch.ones(2048, dtype=BF16, device=DEV)
