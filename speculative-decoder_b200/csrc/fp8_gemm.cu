@@ -361,14 +361,16 @@ __global__ void __launch_bounds__(f8_small_threads(kPerSm), kPerSm)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t stages = a.stages;
 
-  if (threadIdx.x == 0) {
-    for (uint32_t i = 0; i < stages; ++i) {
+  // one barrier per thread: one after another they took half a microsecond
+  if (threadIdx.x < stages + kBufs) {
+    const uint32_t i = threadIdx.x;
+    if (i < stages) {
       mbar_init(&full[i], 1);
       mbar_init(&done[i], 1);
     }
-    for (uint32_t i = 0; i < stages + kBufs; ++i) mbar_init(&sfull[i], 32);
-    for (int i = 0; i < kBufs; ++i) mbar_init(&tempty[i], kF8EpiWarps);
-    abort_flag = 0;
+    mbar_init(&sfull[i], 32);
+    if (i < kBufs) mbar_init(&tempty[i], kF8EpiWarps);
+    if (i == 0) abort_flag = 0;
     fence_mbar_init();
   } else if (warp == 8 && lane == 0) {
     tma_prefetch_desc(&w_map);
@@ -551,7 +553,7 @@ __global__ void __launch_bounds__(f8_small_threads(kPerSm), kPerSm)
         store_warp_tile<__nv_bfloat16, 1>(a, y_map, acc, smem + warp * kF8OutPiece, m0, n0, lane);
       }
     }
-    if (a.rows16 && splits == 1 && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    if (a.rows16 && splits == 1 && lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
   }
   __syncwarp();
   if (splits > 1) {
@@ -640,15 +642,16 @@ __global__ void __launch_bounds__(kF8PairThreads, 1)
   int& abort_flag = bars.abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < kF8PairStages; ++i) {
+  if (threadIdx.x < kF8Slots) {
+    const int i = threadIdx.x;
+    if (i < kF8PairStages) {
       mbar_init(&bars.full[i], 1);
       mbar_init(&bars.done[0][i], 1);
       mbar_init(&bars.done[1][i], 1);
     }
-    for (int i = 0; i < kF8Slots; ++i) mbar_init(&bars.sfull[i], 32);
-    for (int i = 0; i < 4; ++i) mbar_init(&bars.tempty[i >> 1][i & 1], 2 * kF8EpiWarps);
-    abort_flag = 0;
+    mbar_init(&bars.sfull[i], 32);
+    if (i < 4) mbar_init(&bars.tempty[i >> 1][i & 1], 2 * kF8EpiWarps);
+    if (i == 0) abort_flag = 0;
     fence_mbar_init();
   }
   if (warp == 9) f8_tmem_alloc<true>(&bars.tmem_holder, 512);
@@ -835,7 +838,7 @@ __global__ void __launch_bounds__(kF8PairThreads, 1)
       else
         store_warp_tile<__nv_bfloat16, kF8PairPieces>(a, y_map, acc, out_buf, m0, n0, lane);
     }
-    if (a.rows16 && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    if (a.rows16 && lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
     __syncwarp();
   }
   tc_fence_before();
