@@ -316,12 +316,31 @@ SPECB200_DEVINL void store_warp_tile(const F8Args& a, const CUtensorMap& y_map, 
   }
 }
 
+// Adds the partial tiles of a cluster's CTAs in split order, each CTA its share of the outputs:
+// `rows` rows of 128 features with a pitch of 132 floats, at the same address in every CTA.
+SPECB200_DEVINL void add_split_tiles(const F8Args& a, uint32_t tile, int m0, int n0, int rows, int split, int threads) {
+  constexpr int kQuads = kF8Block / 4, kPitch = kF8Block + 4;
+  for (int i = split * threads + threadIdx.x; i < rows * kQuads; i += a.splits * threads) {
+    const int r = i / kQuads, c = (i % kQuads) * 4;
+    if (n0 + c >= a.N) continue;
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    float4 q[kF8MaxSplits];  // all splits' loads in flight
+#pragma unroll
+    for (int p = 0; p < kF8MaxSplits; ++p)
+      if (p < a.splits) q[p] = ld_cluster_f4(tile + (r * kPitch + c) * 4, p);
+#pragma unroll
+    for (int p = 0; p < kF8MaxSplits; ++p)
+      if (p < a.splits) { v[0] += q[p].x; v[1] += q[p].y; v[2] += q[p].z; v[3] += q[p].w; }
+    store_quad(a, static_cast<int64_t>(m0 + r) * a.ldy + n0 + c, a.N - n0 - c, v);
+  }
+}
+
 // ------------------------------------------------------------------------------ small tiles
 // The scales of one group: of a CTA's 128 tokens and of the tile's weight blocks (two for a pair).
-struct F8Scales {
+struct alignas(16) F8Scales {
   float x[kF8TileM], w[4];
 };
-struct F8SmallBarriers {
+struct alignas(16) F8SmallBarriers {
   uint64_t full[kF8MaxStages], done[kF8MaxStages], sfull[kF8MaxStages + 4], tempty[4];
   uint32_t tmem_holder;
   int abort_flag;
@@ -558,24 +577,8 @@ __global__ void __launch_bounds__(f8_small_threads(kPerSm), kPerSm)
   __syncwarp();
   if (splits > 1) {
     cluster_arrive_wait();
-    const int rows = min(kF8TileM, a.M - tile_m);
-    constexpr int kQuads = kF8Block / 4;
-    if (!*reinterpret_cast<volatile int*>(&abort_flag)) {
-      const uint32_t base = smem_u32(smem);
-      for (int i = split * kThreads + threadIdx.x; i < rows * kQuads; i += splits * kThreads) {
-        const int r = i / kQuads, c = (i % kQuads) * 4;
-        if (tile_n + c >= a.N) continue;
-        float v[4] = {0.f, 0.f, 0.f, 0.f};
-        float4 q[kF8MaxSplits];  // all splits' loads in flight, added in split order
-#pragma unroll
-        for (int p = 0; p < kF8MaxSplits; ++p)
-          if (p < splits) q[p] = ld_cluster_f4(base + (r * kPitch + c) * 4, p);
-#pragma unroll
-        for (int p = 0; p < kF8MaxSplits; ++p)
-          if (p < splits) { v[0] += q[p].x; v[1] += q[p].y; v[2] += q[p].z; v[3] += q[p].w; }
-        store_quad(a, static_cast<int64_t>(tile_m + r) * a.ldy + tile_n + c, a.N - tile_n - c, v);
-      }
-    }
+    if (!*reinterpret_cast<volatile int*>(&abort_flag))
+      add_split_tiles(a, smem_u32(smem), tile_m, tile_n, min(kF8TileM, a.M - tile_m), split, kThreads);
     cluster_arrive_wait();  // no CTA leaves while another reads its shared memory
   }
   tc_fence_before();
@@ -583,6 +586,193 @@ __global__ void __launch_bounds__(f8_small_threads(kPerSm), kPerSm)
   if (warp == 9) {
     tc_fence_after();
     f8_tmem_dealloc<false>(*reinterpret_cast<volatile uint32_t*>(&bars.tmem_holder), kBufs * kF8Block);
+  }
+}
+
+// ------------------------------------------------------------------------------ few tokens
+constexpr int kF8FewTokens = 16;  // the least N of an MMA with M = 128
+constexpr int kF8FewThreads = 352;
+constexpr int kF8FewBufs = 4;
+struct alignas(16) F8FewBarriers {
+  uint64_t full[kF8MaxStages], done[kF8MaxStages], sfull[kF8MaxStages + kF8FewBufs], tempty[kF8FewBufs];
+  uint32_t tmem_holder;
+  int abort_flag;
+};
+
+// Up to 16 tokens: decode and verify steps, bound by the stream of weights and by latency. Here
+// the 128 features lie on the TMEM lanes and the tokens are the MMA's N, so that a group costs half the
+// tensor time and every epilogue warp has work: warps 0-3 read the even groups and warps 4-7 the odd
+// ones (w on lane quarter w % 4; a thread owns one feature and all tokens), and their sums meet in
+// shared memory at the end. Producers, MMA warp and the exchange between splits of K are those of the
+// small kernel. 5 x 16384 x 2048 8.2 us (9.1 with the tokens on the lanes), 1 x 6144 x 2048 5.4 (6.3),
+// 5 x 2048 x 8192 6.7 (8.0): 3.0-4.2 TB/s of weights, the rest is the way from launch to the first
+// operands (about 2 us) and from the last ones to the output.
+__global__ void __launch_bounds__(kF8FewThreads, 2)
+    gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map, F8Args a) {
+  constexpr int kTok = kF8FewTokens, kBufs = kF8FewBufs, kProducers = 2;
+  constexpr int kPitch = kF8Block + 4;  // row pitch (floats) of the tile where the sums meet
+  constexpr uint32_t kStageBytes = kF8TileBytes + kTok * kFp8Group;
+  // the ring (1024-byte swizzle atoms), the sums' tile, barriers, scales
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const uint32_t stages = a.stages;
+  float* sums = reinterpret_cast<float*>(smem + stages * kStageBytes);
+  F8FewBarriers& bars = *reinterpret_cast<F8FewBarriers*>(sums + kTok * kPitch);
+  F8Scales* scales = reinterpret_cast<F8Scales*>(&bars + 1);  // stages + kBufs of them
+  uint64_t *full = bars.full, *done = bars.done, *sfull = bars.sfull, *tempty = bars.tempty;
+  int& abort_flag = bars.abort_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x < stages + kBufs) {
+    const uint32_t i = threadIdx.x;
+    if (i < stages) {
+      mbar_init(&full[i], 1);
+      mbar_init(&done[i], 1);
+    }
+    mbar_init(&sfull[i], 32);
+    if (i < kBufs) mbar_init(&tempty[i], 4);
+    if (i == 0) abort_flag = 0;
+    fence_mbar_init();
+  } else if (warp == 8 && lane == 0) {
+    tma_prefetch_desc(&w_map);
+    tma_prefetch_desc(&x_map);
+  }
+  __syncthreads();
+
+  const int splits = a.splits, split = static_cast<int>(blockIdx.x) % splits;
+  const int tile_n = static_cast<int>(blockIdx.x) / splits * kF8Block;
+  const int kb0 = static_cast<int>(static_cast<int64_t>(a.kblocks) * split / splits);
+  const int groups = static_cast<int>(static_cast<int64_t>(a.kblocks) * (split + 1) / splits) - kb0;
+
+  if (warp == 8 || warp == 10) {
+    pdl_wait();
+    const float* sx = a.xs + static_cast<int64_t>(lane) * a.kblocks + kb0;
+    const float* sw = a.ws + static_cast<int64_t>(tile_n / kF8Block) * a.kblocks + kb0;
+    const int me = warp == 8 ? 0 : 1;
+    auto load = [&](int g, uint32_t st) {
+      if (lane == 0) {
+        uint8_t* s = smem + st * kStageBytes;
+        mbar_arrive_expect_tx(&full[st], kStageBytes);
+        tma_load_2d(s, &w_map, &full[st], (kb0 + g) * kFp8Group, tile_n);
+        tma_load_2d(s + kF8TileBytes, &x_map, &full[st], (kb0 + g) * kFp8Group, 0);
+      }
+      __syncwarp();
+    };
+    auto fetch = [&](int g, uint32_t slot) {
+      if (lane < a.M) copy_async_4(&scales[slot].x[lane], sx + g);
+      if (lane == 0) copy_async_4(&scales[slot].w[0], sw + g);
+      copy_async_arrive(&sfull[slot]);
+    };
+    // as in the small kernel
+    const int first = min(groups, static_cast<int>(stages));
+    for (int g = me; g < first; g += kProducers) load(g, g);
+    for (int g = me; g < first; g += kProducers) fetch(g, g);
+    uint32_t st = 0, phase = 0, slot = stages;
+    for (int g = first; g < groups; ++g) {
+      if (g % kProducers == me) {
+        if (!wait_warp(&done[st], phase, a.status, &abort_flag)) {
+          for (int i = max(0, g - static_cast<int>(stages)); i < g; ++i)
+            if (lane == 0 && i % kProducers == me)
+              mbar_wait_bounded(&full[i % stages], (i / stages) & 1, a.status, nullptr);
+          break;
+        }
+        load(g, st);
+        fetch(g, slot);
+      }
+      if (++st == stages) { st = 0; phase ^= 1; }
+      if (++slot == stages + kBufs) slot = 0;
+    }
+    __syncwarp();
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    pdl_launch_dependents();
+  } else if (warp == 9) {
+    f8_tmem_alloc<false>(&bars.tmem_holder, kBufs * kTok);
+    tc_fence_before();
+    __syncwarp();
+    tc_fence_after();
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&bars.tmem_holder);
+    pdl_launch_dependents();  // as in the small kernel, after the allocation
+    constexpr uint32_t idesc = umma_idesc_e4m3(kF8Block, kTok);
+    const uint32_t leader = elect_leader();
+    const uint64_t dw0 = umma_desc_sw128(smem_u32(smem)), dx0 = umma_desc_sw128(smem_u32(smem + kF8TileBytes));
+    uint32_t st = 0, phase = 0, buf = 0, acc_phase = 0;
+    for (int g = 0; g < groups; ++g) {
+      if (!wait_warp<true>(&tempty[buf], acc_phase ^ 1, &full[st], phase, a.status, &abort_flag)) break;
+      tc_fence_after();
+      const uint64_t at = static_cast<uint64_t>(st * (kStageBytes >> 4));
+      umma_group_e4m3<false>(leader, tmem + buf * kTok, dw0 + at, dx0 + at, idesc, &done[st]);
+      if (++st == stages) { st = 0; phase ^= 1; }
+      if (++buf == kBufs) { buf = 0; acc_phase ^= 1; }
+    }
+  } else {
+    pdl_wait();
+    const int quarter = warp & 3, odd = warp >> 2, feature = quarter * 32 + lane;
+    float acc[kTok];
+#pragma unroll
+    for (int i = 0; i < kTok; ++i) acc[i] = 0.f;
+    uint32_t st = odd, phase = 0, slot = odd, slot_phase = 0, buf = odd, tbase = 0;
+    bool ok = true;
+    for (int g = odd; g < groups; g += 2) {
+      ok = wait_warp<true>(&done[st], phase, &sfull[slot], slot_phase, a.status, &abort_flag);
+      if (!ok) break;
+      tc_fence_after();
+      if (g == odd) {
+        tbase = *reinterpret_cast<volatile uint32_t*>(&bars.tmem_holder) + (static_cast<uint32_t>(quarter * 32) << 16);
+        pdl_launch_dependents();
+      }
+      const F8Scales& sc = scales[slot];
+      const float w = sc.w[0];
+      uint32_t r[kTok];
+      tmem_ld<kTok>(tbase + buf * kTok, r);
+      float f[kTok];
+#pragma unroll
+      for (int i = 0; i < kTok; i += 4) {
+        const float4 x = *reinterpret_cast<const float4*>(&sc.x[i]);
+        f[i] = x.x * w; f[i + 1] = x.y * w; f[i + 2] = x.z * w; f[i + 3] = x.w * w;
+      }
+      tmem_ld_wait();
+      tc_fence_before();  // read: a later group may overwrite it
+      if (lane == 0) mbar_arrive(&tempty[buf]);
+#pragma unroll
+      for (int i = 0; i < kTok; ++i) acc[i] = fmaf(__uint_as_float(r[i]), f[i], acc[i]);
+      st += 2;
+      if (st >= stages) { st -= stages; phase ^= 1; }
+      slot += 2;
+      if (slot >= stages + kBufs) { slot -= stages + kBufs; slot_phase ^= 1; }
+      buf ^= 2;
+    }
+    // the odd groups' sums to shared memory, the even groups' added to them
+    if (odd) {
+#pragma unroll
+      for (int i = 0; i < kTok; ++i)
+        if (i < a.M) sums[i * kPitch + feature] = acc[i];
+    }
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+    if (!odd && ok) {
+      const int n = tile_n + feature;
+#pragma unroll
+      for (int i = 0; i < kTok; ++i) {
+        if (i >= a.M) break;
+        const float v = acc[i] + sums[i * kPitch + feature];
+        if (splits > 1)
+          sums[i * kPitch + feature] = v;
+        else if (n < a.N && a.out_f32)
+          static_cast<float*>(a.y)[static_cast<int64_t>(i) * a.ldy + n] = v;
+        else if (n < a.N)
+          static_cast<__nv_bfloat16*>(a.y)[static_cast<int64_t>(i) * a.ldy + n] = __float2bfloat16_rn(v);
+      }
+    }
+  }
+  __syncwarp();
+  if (splits > 1) {
+    cluster_arrive_wait();
+    if (!*reinterpret_cast<volatile int*>(&abort_flag)) add_split_tiles(a, smem_u32(sums), 0, tile_n, a.M, split, kF8FewThreads);
+    cluster_arrive_wait();  // no CTA leaves while another reads its shared memory
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    f8_tmem_dealloc<false>(*reinterpret_cast<volatile uint32_t*>(&bars.tmem_holder), kBufs * kTok);
   }
 }
 
@@ -853,7 +1043,8 @@ __global__ void __launch_bounds__(kF8PairThreads, 1)
 // ------------------------------------------------------------------------------ host side
 struct F8Plan {
   bool pair;
-  int per_sm;  // CTAs per SM that the small kernel is cut for
+  bool few;
+  int per_sm;  // CTAs per SM that the ring (and the small kernel) is cut for
   int splits, stages, box_rows;
   int kblocks, m_tiles, n_tiles;
   size_t ring, smem;
@@ -880,12 +1071,22 @@ F8Plan plan_fp8(int M, int N, int K) {
   // A group takes a CTA alone on its SM about 0.29 us, and the exchange of partial tiles 1.4-2.5 us
   // (more for more tokens): K is split where it is long enough to win that back, at most four
   // ways, and only while all clusters find room at once (four CTAs of an SM each do not fill every
-  // GPC). Decode 1 x 6144 x 2048: 6.9 us unsplit, 6.5 split in two; 320 x 2048 x 8192: 22.1 and 15.5;
-  // 320 x 2048 x 2048: 7.5 and 8.0.
+  // GPC). 5 x 2048 x 2048: 5.0 us unsplit, 4.5 and 4.2 split in two and four; 320 x 2048 x 8192: 22.1
+  // and 15.5; 320 x 2048 x 2048: 7.5 and 8.0.
   p.per_sm = tiles <= 148 ? 1 : 2;
   if (p.kblocks >= (p.box_rows <= 32 ? 16 : 24))
     while (p.splits < kF8MaxSplits && tiles * p.splits * 2 <= (p.splits == 1 ? 148 : 128) && p.kblocks >= 8 * p.splits)
       p.splits *= 2;
+  // 32 tokens on the MMA's N were slower than on the lanes (32 x 16384 x 2048: 10.6 against 9.0 us).
+  if (M <= kF8FewTokens) {
+    p.few = true;
+    p.box_rows = kF8FewTokens;
+    const size_t stage = kF8TileBytes + kF8FewTokens * kFp8Group;
+    const size_t fixed = kF8FewTokens * (kF8Block + 4) * sizeof(float) + sizeof(F8FewBarriers) + kF8FewBufs * sizeof(F8Scales);
+    p.stages = static_cast<int>(std::min<size_t>(kF8MaxStages, ((p.per_sm == 1 ? 227 : 113) * 1024 - fixed) / (stage + sizeof(F8Scales))));
+    p.smem = fixed + p.stages * (stage + sizeof(F8Scales));
+    return p;
+  }
   const size_t x_bytes = static_cast<size_t>(p.box_rows) * kFp8Group, stage = kF8TileBytes + x_bytes;
   // An MMA reads 128 token rows: with fewer in a box it runs on into the next stage, whose lanes
   // are never read back; the last stage needs that much room behind it.
@@ -914,8 +1115,9 @@ cudaError_t prepare_fp8(K kernel, std::atomic<bool> (&ready)[kF8MaxDevices]) {
 
 cudaError_t launch_fp8(const F8Plan& p, const CUtensorMap& wm, const CUtensorMap& xm, const CUtensorMap& ym, const F8Args& a,
                        cudaStream_t s) {
-  static std::atomic<bool> ready[3][kF8MaxDevices];
-  const cudaError_t e = p.pair          ? prepare_fp8(gemm_fp8_pair_kernel, ready[0])
+  static std::atomic<bool> ready[4][kF8MaxDevices];
+  const cudaError_t e = p.few           ? prepare_fp8(gemm_fp8_few_kernel, ready[3])
+                        : p.pair          ? prepare_fp8(gemm_fp8_pair_kernel, ready[0])
                         : p.per_sm == 1 ? prepare_fp8(gemm_fp8_small_kernel<1>, ready[1])
                                         : prepare_fp8(gemm_fp8_small_kernel<2>, ready[2]);
   if (e != cudaSuccess) return e;
@@ -923,7 +1125,7 @@ cudaError_t launch_fp8(const F8Plan& p, const CUtensorMap& wm, const CUtensorMap
   const int cluster = p.pair ? 2 : p.splits;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>((p.pair ? std::min<int64_t>(tiles, 74) : tiles) * cluster));
-  cfg.blockDim = dim3(p.pair ? kF8PairThreads : f8_small_threads(p.per_sm));
+  cfg.blockDim = dim3(p.few ? kF8FewThreads : p.pair ? kF8PairThreads : f8_small_threads(p.per_sm));
   cfg.dynamicSmemBytes = p.smem;
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
@@ -935,6 +1137,7 @@ cudaError_t launch_fp8(const F8Plan& p, const CUtensorMap& wm, const CUtensorMap
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = cluster > 1 ? 2 : 1;
+  if (p.few) return cudaLaunchKernelEx(&cfg, gemm_fp8_few_kernel, wm, xm, a);
   return p.pair ? cudaLaunchKernelEx(&cfg, gemm_fp8_pair_kernel, wm, xm, ym, a)
                 : p.per_sm == 1 ? cudaLaunchKernelEx(&cfg, gemm_fp8_small_kernel<1>, wm, xm, ym, a)
                                 : cudaLaunchKernelEx(&cfg, gemm_fp8_small_kernel<2>, wm, xm, ym, a);
@@ -970,7 +1173,7 @@ extern "C" int specb200_linear_fp8(const void* x, int64_t ldx, const float* x_sc
   CUtensorMap ym = {};
   const int esize = out_f32 ? 4 : 2;
   const bool y_rows16 = fp8_aligned(y, 16) && (ldy * esize) % 16 == 0;
-  if (p.splits == 1 && y_rows16 && !make_tmap_out_2d(&ym, y, out_f32 != 0, N, M, ldy * esize, 128 / esize, 32))
+  if (!p.few && p.splits == 1 && y_rows16 && !make_tmap_out_2d(&ym, y, out_f32 != 0, N, M, ldy * esize, 128 / esize, 32))
     return specb200_set_error(SPECB200_ERR_ARG, "linear_fp8: TMA descriptor");
   F8Args a = {};
   a.M = M;

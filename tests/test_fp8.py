@@ -468,7 +468,7 @@ def test_silu_mul_far_gates():
 
 # ---------------------------------------------------------------- linear
 LINEAR = [(1, 1, 1), (1, 16, 16), (1, 128, 128), (2, 130, 129), (5, 960, 576), (8, 256, 2048), (9, 6144, 2048),
-          (33, 2048, 8192), (64, 1000, 1000), (127, 300, 200), (128, 128, 640), (129, 257, 384), (320, 2048, 1024),
+          (33, 2048, 8192), (16, 500, 4096), (17, 500, 4096), (15, 40000, 256), (64, 1000, 1000), (127, 300, 200), (128, 128, 640), (129, 257, 384), (320, 2048, 1024),
           (513, 1024, 300), (1000, 1536, 576), (2049, 4100, 520), (3000, 5000, 130)]
 
 
@@ -544,9 +544,10 @@ def test_linear_is_the_same_every_time_and_in_any_batch():
     assert torch.equal(ops.linear_fp8(x[2:5], xs[2:5], w, ws), y[2:5])
 
 
-# one shape for each way a product is split over CTAs: one tile per SM, K split in two and four, two
-# tiles per SM, pairs with a partial last wave, pairs with an odd number of groups
-PLANS = [(40, 900, 512), (300, 2048, 4096), (3, 2048, 2048), (128, 25600, 256), (700, 12000, 256), (2000, 5000, 384)]
+# one shape for each way a product is split over CTAs: up to 16 tokens (odd number of groups, K split in
+# four, two tiles per SM), one tile per SM, K split in two and four, two tiles per SM, pairs with a
+# partial last wave, pairs with an odd number of groups
+PLANS = [(9, 900, 1152), (16, 2048, 8192), (5, 25600, 640), (17, 2048, 2048), (40, 900, 512), (300, 2048, 4096), (3, 2048, 2048), (128, 25600, 256), (700, 12000, 256), (2000, 5000, 384)]
 
 
 @pytest.mark.gpu
