@@ -5,8 +5,6 @@
 // 448 is e4m3's largest value. The floor keeps 1 / s finite for groups of zeros; a NaN or an
 // infinity in a group makes its scale NaN or infinite and so stays visible in every product.
 #pragma once
-#include <cuda_fp8.h>
-
 #include "common.cuh"
 
 namespace specb200 {
@@ -23,16 +21,6 @@ SPECB200_DEVINL float max_nan(float a, float b) {
 }
 SPECB200_DEVINL float max_mag(float m, float x) { return max_nan(m, fabsf(x)); }
 SPECB200_DEVINL float floor_amax(float amax) { return amax < kFp8MinAmax ? kFp8MinAmax : amax; }
-
-// Eight fp32 values as e4m3, rounded to nearest even; finite values beyond 448 (a group's
-// maximum can exceed it by an ulp) saturate, NaN stays NaN.
-SPECB200_DEVINL uint2 pack_e4m3(const float (&f)[8]) {
-  uint32_t h[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    h[i] = __nv_cvt_float2_to_fp8x2(make_float2(f[2 * i], f[2 * i + 1]), __NV_SATFINITE, __NV_E4M3);
-  return make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
-}
 
 inline bool fp8_aligned(const void* p, uint64_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 

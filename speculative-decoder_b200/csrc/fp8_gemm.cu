@@ -5,12 +5,13 @@
 // The inner sum runs on the tensor cores (tcgen05.mma kind::f8f6f4, fp32 accumulator in TMEM);
 // its 128 products of one group share one pair of scales, so each group's partial tile is read
 // back and added to fp32 registers with the factor sx * sw, while the MMAs of the next group run
-// into another TMEM buffer. Tokens lie on the TMEM lanes: a thread owns one token and features of
+// into another TMEM buffer. Where tokens lie on the TMEM lanes a thread owns one token and features of
 // one weight block, so the factor of a group is one number per thread. Operands come by TMA, K-major
-// with the 128-byte swizzle (one atom is one group). Two kernels:
+// with the 128-byte swizzle (one atom is one group). Three kernels:
 //
-// - gemm_fp8_small_kernel: a CTA computes one tile of 128 tokens x 128 features, two CTAs per SM.
-//   With few tiles K is split over the CTAs of a cluster: each leaves its partial tile in its own
+// - gemm_fp8_few_kernel: up to 16 tokens x 128 features per CTA, features on the lanes.
+// - gemm_fp8_small_kernel: a CTA computes one tile of 128 tokens x 128 features, one or two CTAs per
+//   SM. In either, with few tiles K is split over the CTAs of a cluster: each leaves its partial tile in its own
 //   shared memory and the cluster adds them through distributed shared memory in split order, so
 //   results do not depend on scheduling and no workspace exists that two calls could share.
 // - gemm_fp8_pair_kernel: a pair of CTAs (cta_group::2) walks over tiles of 256 tokens x 256
@@ -32,7 +33,9 @@ constexpr int kF8MaxStages = 12;
 constexpr int kF8MaxDevices = 64;
 constexpr int kF8EpiWarps = 8;
 // The small kernel is cut for one or two CTAs per SM: alone a CTA has four TMEM buffers, twice the
-// ring, a second producer warp and registers to read ahead.
+// ring, a second producer warp and registers to read ahead (64 x 6144 x 2048: 7.4 us against 9.6; 320 x
+// 2048 x 8192 without a split of K: 22.3 against 34.6). Two to an SM hide each other's start and end where there are
+// more tiles than SMs.
 __host__ __device__ constexpr int f8_small_threads(int per_sm) { return per_sm == 1 ? 352 : 320; }
 __host__ __device__ constexpr int f8_small_bufs(int per_sm) { return per_sm == 1 ? 4 : 2; }
 constexpr int kF8PairThreads = 384;
@@ -148,13 +151,6 @@ SPECB200_DEVINL void tmem_ld<16>(uint32_t taddr, uint32_t (&r)[16]) {
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
         "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(taddr));
-}
-
-template <>
-SPECB200_DEVINL void tmem_ld<8>(uint32_t taddr, uint32_t (&r)[8]) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-               : "r"(taddr));
 }
 
 SPECB200_DEVINL void cluster_arrive_wait() {
@@ -604,8 +600,8 @@ struct alignas(16) F8FewBarriers {
 // tensor time and every epilogue warp has work: warps 0-3 read the even groups and warps 4-7 the odd
 // ones (w on lane quarter w % 4; a thread owns one feature and all tokens), and their sums meet in
 // shared memory at the end. Producers, MMA warp and the exchange between splits of K are those of the
-// small kernel. 5 x 16384 x 2048 8.2 us (9.1 with the tokens on the lanes), 1 x 6144 x 2048 5.4 (6.3),
-// 5 x 2048 x 8192 6.7 (8.0): 3.0-4.2 TB/s of weights, the rest is the way from launch to the first
+// small kernel. 5 x 16384 x 2048 8.2 us (9.2 with the tokens on the lanes), 1 x 6144 x 2048 5.5 (6.3),
+// 5 x 2048 x 8192 6.7 (8.0): 2.3-4.1 TB/s of weights, the rest is the way from launch to the first
 // operands (about 2 us) and from the last ones to the output.
 __global__ void __launch_bounds__(kF8FewThreads, 2)
     gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map, F8Args a) {
@@ -816,7 +812,7 @@ struct F8TileWalk {
 // all): half h holds features 64 h..64 h + 63 of either weight block, so that each epilogue thread reads 64
 // columns of a half. What a buffer costs besides its MMAs -- the commit's and the release's way
 // between warps and CTAs, the read -- then hides behind three other buffers' MMAs; with one buffer per group it
-// did not (8192 x 16384 x 2048: 253 us).
+// did not (8192 x 16384 x 2048: 266 us against 286; 245 in the end).
 // Warps 0-7 read back (w on TMEM lane quarter w % 4, weight block w / 4), warps 9
 // and 10 of the pair's first CTA tcgen05.mma for both; warps 8 and 11 load operands and scales. Either
 // kind takes turns: MMAs issue in order and block the warp while the tensor cores are busy, and a
@@ -1042,8 +1038,7 @@ __global__ void __launch_bounds__(kF8PairThreads, 1)
 
 // ------------------------------------------------------------------------------ host side
 struct F8Plan {
-  bool pair;
-  bool few;
+  bool pair, few;
   int per_sm;  // CTAs per SM that the ring (and the small kernel) is cut for
   int splits, stages, box_rows;
   int kblocks, m_tiles, n_tiles;
@@ -1059,7 +1054,8 @@ F8Plan plan_fp8(int M, int N, int K) {
   p.splits = 1;
   const int64_t tiles = static_cast<int64_t>(p.m_tiles) * p.n_tiles;
   // More than one tile per SM and tokens for pairs: pairs, although their last wave may be partial
-  // (512 x 16384 x 2048: 21.1 us against 25.4 on small tiles; 160 x 16384 x 2048: 13.1 against 12.7).
+  // (512 x 16384 x 2048: 21.0 us against 25.2 on small tiles; 320 x 16384 x 2048: 19.8 and 21.6; 160 x
+  // 16384 x 2048: 13.0 and 12.9).
   p.pair = M > kF8TileM && tiles > 148;
   if (p.pair) {
     p.m_tiles = (p.m_tiles + 1) / 2;
@@ -1071,8 +1067,8 @@ F8Plan plan_fp8(int M, int N, int K) {
   // A group takes a CTA alone on its SM about 0.29 us, and the exchange of partial tiles 1.4-2.5 us
   // (more for more tokens): K is split where it is long enough to win that back, at most four
   // ways, and only while all clusters find room at once (four CTAs of an SM each do not fill every
-  // GPC). 5 x 2048 x 2048: 5.0 us unsplit, 4.5 and 4.2 split in two and four; 320 x 2048 x 8192: 22.1
-  // and 15.5; 320 x 2048 x 2048: 7.5 and 8.0.
+  // GPC; four-CTA clusters find room for 132). 5 x 2048 x 2048: 5.0 us unsplit, 4.2 split in four; 5 x
+  // 2048 x 8192: 15.2 and 6.7; 320 x 2048 x 8192: 22.3 and 15.0 in two; but 320 x 2048 x 2048: 7.5 and 8.0.
   p.per_sm = tiles <= 148 ? 1 : 2;
   if (p.kblocks >= (p.box_rows <= 32 ? 16 : 24))
     while (p.splits < kF8MaxSplits && tiles * p.splits * 2 <= (p.splits == 1 ? 148 : 128) && p.kblocks >= 8 * p.splits)

@@ -2,9 +2,11 @@
 // with the residual update in front, and SiLU(gate) * up. Everything between the inputs and the
 // e4m3 rounding is fp32; the only other rounding is the residual stream's own element type.
 //
-// All are bound by memory: each input is read once, 16 bytes per lane, and each output written
-// once. A group of 128 columns is held by 16 lanes with 8 elements each, so its maximum is four
-// shuffles and its scale is written by the group's first lane.
+// All are bound by memory: each input is read once, in loads of 32 bytes per lane, and each output
+// written once, 16 bytes of e4m3 per lane. A group of 128 columns is held by 8 lanes with 16 elements
+// each, so its maximum is three shuffles and its scale is written by the group's first lane.
+#include <cuda_fp8.h>
+
 #include <algorithm>
 
 #include "fp8.cuh"
@@ -129,7 +131,8 @@ SPECB200_DEVINL void store16(T* p, int valid, int align, const Raw16<T>& r) {
     }
   }
 }
-// e4m3(f * inv), 16 of a row.
+// e4m3(f * inv), 16 of a row, rounded to nearest even. Finite values beyond 448 (a group's maximum can
+// exceed it by an ulp) saturate, NaN stays NaN.
 SPECB200_DEVINL void store_q16(uint8_t* p, int valid, int align, const f32x2 (&f)[8], float inv) {
   const f32x2 inv2 = pack2(inv, inv);
   uint32_t v[4];
@@ -296,9 +299,10 @@ struct NormArgs {
 constexpr int kNormMaxChunks = 4;                            // groups of a row per 8 lanes
 constexpr int kNormMaxWidth = kNormMaxChunks * 64 * kFp8Group;  // 64 octets: 512 threads
 
-// CTAs per SM that the registers are cut for. 32768 x 2048 bf16 with delta, loads ahead: 72.9 us at 3
-// CTAs (98% of the measured bandwidth), 82.7 at 2, and 80.3 at 4 without room for loads ahead; fp32
-// 16384 x 2048: 68.7 at 2, 74.2 at 3. 8192 x 8192 bf16 (two groups per octet): 82.4 at 3, 88.8 at 2.
+// CTAs per SM that the registers are cut for. 32768 x 2048 bf16 with delta, loads ahead: 71.5 us at 3
+// CTAs (floor 71.9 at the measured copy bandwidth), 81.8 at 2, and 86.2 at 4, which leaves no room for
+// loads ahead; fp32 16384 x 2048: 67.1 at 2, 80.5 at 3. 8192 x 8192 bf16 (two groups per octet): 80.7
+// at 3, 84.4 at 2, 87.4 at 4.
 template <typename T, int kChunks>
 constexpr int kNormCtas = kChunks == 4 ? 1 : kChunks == 2 ? 3 : sizeof(T) == 2 ? 3 : 2;
 
@@ -445,19 +449,24 @@ cudaError_t launch_silu_mul(RowArgs a, cudaStream_t s) {
   return launch_kernel(quantize_rows_kernel<T, true>, dim3(row_ctas(a)), dim3(kRowThreads), 0, s, true, a);
 }
 
-// As many CTAs as the 148 SMs hold at once, each on every grid-th set of rows.
-template <typename K>
+// As many CTAs as the 148 SMs hold at once, each on every grid-th set of rows. Up to the number that
+// the kernel's registers are cut for every row set has its CTA, and the driver need not be asked.
+template <int kCtas, typename K>
 cudaError_t launch_filled(K kernel, const NormArgs& a, int threads, cudaStream_t s) {
-  int per_sm = 0;
-  const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, 0);
-  if (e != cudaSuccess) return e;
-  return launch_kernel(kernel, dim3(std::min((a.M - 1) / a.rows + 1, 148 * std::max(1, per_sm))), dim3(threads), 0, s, true, a);
+  const int wanted = (a.M - 1) / a.rows + 1;
+  int per_sm = kCtas;
+  if (wanted > 148 * kCtas) {
+    const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, 0);
+    if (e != cudaSuccess) return e;
+  }
+  return launch_kernel(kernel, dim3(std::min(wanted, 148 * std::max(1, per_sm))), dim3(threads), 0, s, true, a);
 }
 template <typename T, int kChunks>
 cudaError_t launch_norm_kernel(const NormArgs& a, int octets, cudaStream_t s) {
+  constexpr int kCtas = kNormCtas<T, kChunks>;
   const int threads = (octets * 8 + 31) / 32 * 32;
-  return a.delta ? launch_filled(rmsnorm_fp8_kernel<T, kChunks, true>, a, threads, s)
-                 : launch_filled(rmsnorm_fp8_kernel<T, kChunks, false>, a, threads, s);
+  return a.delta ? launch_filled<kCtas>(rmsnorm_fp8_kernel<T, kChunks, true>, a, threads, s)
+                 : launch_filled<kCtas>(rmsnorm_fp8_kernel<T, kChunks, false>, a, threads, s);
 }
 
 template <typename T>

@@ -227,6 +227,15 @@ Rows operand_of(const at::Tensor& x, const char* what) {
   return r;
 }
 
+// The status word, with the interpreter free for other threads while the stream runs.
+int wait_for(const at::Tensor& status) {
+  struct Released {
+    PyThreadState* state = PyEval_SaveThread();
+    ~Released() { PyEval_RestoreThread(state); }
+  } released;
+  return status.item<int>();
+}
+
 PyObject* linear(PyObject* const* args) {
   const char* where = "linear_fp8";
   const at::Tensor& x = tensor(args[0], where);
@@ -261,7 +270,7 @@ PyObject* linear(PyObject* const* args) {
                                         check ? static_cast<int32_t*>(status.data_ptr()) : nullptr, here.stream));
   }
   if (check) {
-    const int code = status.item<int>();
+    const int code = wait_for(status);
     if (code == SPECB200_ERR_TIMEOUT) throw Refusal{PyExc_RuntimeError, text(where, ": a device-side wait gave up (timeout)")};
     if (code != SPECB200_OK) throw Refusal{PyExc_RuntimeError, text(where, ": device status ", code)};
   }
