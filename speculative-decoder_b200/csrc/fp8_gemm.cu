@@ -298,14 +298,25 @@ SPECB200_DEVINL void store_warp_tile(const F8Args& a, const CUtensorMap& y_map, 
     }
     for (int c = c0; c < c0 + kRound; c += kPiece) {
       if (by_tma(c)) continue;
-      const int n = n0 + c + (lane & 7) * kUnit;
-      for (int r = lane >> 3; r < 32; r += 4) {
-        const uint4 q = *reinterpret_cast<const uint4*>(bufs + (c - c0) / kPiece * kF8OutPiece + r * 128 + ((lane ^ r) & 7) * 16);
-        const T* e = reinterpret_cast<const T*>(&q);
-        T* y = static_cast<T*>(a.y) + static_cast<int64_t>(m0 + r) * a.ldy + n;
-#pragma unroll
-        for (int j = 0; j < kUnit; ++j)
-          if (m0 + r < a.M && n + j < a.N) y[j] = e[j];
+      // a row at a time, four bytes per lane: one element, or the pair that starts on a 4-byte boundary
+      const int rows = min(32, a.M - m0), left = a.N - n0 - c;
+      const uint8_t* piece = bufs + (c - c0) / kPiece * kF8OutPiece + (lane & 3) * 4;
+      T* y = static_cast<T*>(a.y) + static_cast<int64_t>(m0) * a.ldy + n0 + c;
+#pragma unroll 16
+      for (int r = 0; r < rows; ++r, y += a.ldy) {
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(piece + r * 128 + (((lane >> 2) ^ r) & 7) * 16);
+        if constexpr (sizeof(T) == 4) {
+          if (lane < left) y[lane] = __uint_as_float(w);
+        } else {
+          const int odd = static_cast<int>(reinterpret_cast<uintptr_t>(y) >> 1) & 1, n = 2 * lane + odd;
+          const uint32_t next = __shfl_down_sync(0xffffffffu, w, 1);
+          unsigned short* o = reinterpret_cast<unsigned short*>(y);
+          if (n + 1 < min(left, kPiece))
+            *reinterpret_cast<uint32_t*>(o + n) = odd ? (w >> 16) | (next << 16) : w;
+          else if (n < left)
+            o[n] = static_cast<unsigned short>(odd ? w >> 16 : w);
+          if (odd && lane == 0 && left > 0) o[0] = static_cast<unsigned short>(w);
+        }
       }
     }
     __syncwarp();

@@ -44,18 +44,48 @@ SPECB200_DEVINL f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
   return r;
 }
 
-// Sixteen consecutive elements of a row, in the form they have in memory. align: every row starts
-// on a boundary of that many bytes: 32 takes 256-bit loads, 16 takes 128-bit ones, less one load
-// per element.
+// Sixteen consecutive elements of a row, in the form they have in memory.
 template <typename T>
 struct Raw16 {
   uint32_t v[4 * sizeof(T)];
 };
-template <typename T>
-SPECB200_DEVINL void load16(Raw16<T>& r, const T* p, int valid, int align) {
-  constexpr int kWords = 4 * sizeof(T);
-  if (align >= 16 && valid >= 16) {
-    const char* b = reinterpret_cast<const char*>(p);
+// The same as they are loaded. kAny = false: rows start on 16-byte boundaries; one or two 256-bit
+// loads (or 128-bit ones, align 16). kAny = true: rows start anywhere, and what is loaded is the
+// 16-byte units that the elements lie in, `shift` bytes of the first one ahead of them (16384 x 2050
+// bf16: quantize 23.7 us, RMSNorm 90; with a load per element 38 and 207).
+template <typename T, bool kAny>
+struct Loaded16 {
+  uint32_t v[4 * sizeof(T) + (kAny ? 4 : 0)];
+  uint32_t shift;
+};
+// first, end: the bytes of the whole tensor, beyond which no unit is read.
+template <typename T, bool kAny>
+SPECB200_DEVINL void load16(Loaded16<T, kAny>& r, const T* p, int valid, int align, const void* first, const void* end) {
+  constexpr int kWords = 4 * sizeof(T), kAll = kAny ? kWords + 4 : kWords;
+  const char* b = reinterpret_cast<const char*>(p);
+  r.shift = 0;
+  if constexpr (kAny) {
+    const int shift = static_cast<int>(reinterpret_cast<uintptr_t>(p) & 15), bytes = min(valid, 16) * static_cast<int>(sizeof(T)) + shift;
+    b -= shift;
+    if (valid > 0 && b >= first && b + (bytes + 15) / 16 * 16 <= end) {
+      r.shift = shift;
+#pragma unroll
+      for (int i = 0; i < kAll; i += 4) {
+        uint4 q = make_uint4(0, 0, 0, 0);
+        if (4 * i < bytes) q = *reinterpret_cast<const uint4*>(b + 4 * i);
+        r.v[i] = q.x; r.v[i + 1] = q.y; r.v[i + 2] = q.z; r.v[i + 3] = q.w;
+      }
+      if (valid < 16) {  // what follows the row's end
+#pragma unroll
+        for (int i = 0; i < kAll; ++i) {
+          const int left = bytes - 4 * i;
+          if (left <= 0) r.v[i] = 0;
+          if (left == 2) r.v[i] &= 0xffffu;
+        }
+      }
+      return;
+    }
+  } else if (align >= 16 && valid >= 16) {
     if (align >= 32) {
 #pragma unroll
       for (int i = 0; i < kWords; i += 8)
@@ -73,7 +103,7 @@ SPECB200_DEVINL void load16(Raw16<T>& r, const T* p, int valid, int align) {
     return;
   }
 #pragma unroll
-  for (int i = 0; i < kWords; ++i) r.v[i] = 0;
+  for (int i = 0; i < kAll; ++i) r.v[i] = 0;
   if (valid <= 0) return;  // lanes behind a row's end: their warp need not go through the single loads
 #pragma unroll
   for (int i = 0; i < kWords; ++i) {
@@ -85,6 +115,35 @@ SPECB200_DEVINL void load16(Raw16<T>& r, const T* p, int valid, int align) {
       r.v[i] = i < valid ? reinterpret_cast<const uint32_t*>(p)[i] : 0;
     }
   }
+}
+// w[0..kOut) = the words that start `bytes` (0..15, even) into w.
+template <int kOut, bool kHalves>
+SPECB200_DEVINL void shift_words(uint32_t (&w)[kOut + 4], uint32_t bytes) {
+#pragma unroll
+  for (int i = 0; i < kOut + 2; ++i) w[i] = bytes & 8 ? w[i + 2] : w[i];
+#pragma unroll
+  for (int i = 0; i < kOut + 1; ++i) w[i] = bytes & 4 ? w[i + 1] : w[i];
+  if constexpr (kHalves) {
+#pragma unroll
+    for (int i = 0; i < kOut; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], (bytes & 2) * 8);
+  }
+}
+template <typename T, bool kAny>
+SPECB200_DEVINL Raw16<T> aligned16(const Loaded16<T, kAny>& l) {
+  constexpr int kWords = 4 * sizeof(T);
+  Raw16<T> r;
+  if constexpr (kAny) {
+    uint32_t w[kWords + 4];
+#pragma unroll
+    for (int i = 0; i < kWords + 4; ++i) w[i] = l.v[i];
+    shift_words<kWords, sizeof(T) == 2>(w, l.shift);
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) r.v[i] = w[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) r.v[i] = l.v[i];
+  }
+  return r;
 }
 template <typename T>
 SPECB200_DEVINL void unpack16(const Raw16<T>& r, f32x2 (&f)[8]) {
@@ -113,22 +172,73 @@ SPECB200_DEVINL Raw16<T> round16(const f32x2 (&f)[8]) {
   }
   return r;
 }
-template <typename T>
-SPECB200_DEVINL void store16(T* p, int valid, int align, const Raw16<T>& r) {
-  constexpr int kWords = 4 * sizeof(T);
-  if (align >= 16 && valid >= 16) {
-#pragma unroll
-    for (int i = 0; i < kWords; i += 4)
-      reinterpret_cast<uint4*>(p)[i / 4] = make_uint4(r.v[i], r.v[i + 1], r.v[i + 2], r.v[i + 3]);
+// The first `bytes` (0..16) of w to p, which is on a 16-byte boundary.
+SPECB200_DEVINL void store_unit(char* p, int bytes, uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3) {
+  if (bytes >= 16) {
+    *reinterpret_cast<uint4*>(p) = make_uint4(w0, w1, w2, w3);
     return;
   }
+  if (bytes <= 0) return;
+  if (bytes & 8) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(w0, w1);
+    w0 = w2; w1 = w3;
+    p += 8;
+  }
+  if (bytes & 4) {
+    *reinterpret_cast<uint32_t*>(p) = w0;
+    w0 = w1;
+    p += 4;
+  }
+  if (bytes & 2) {
+    *reinterpret_cast<unsigned short*>(p) = static_cast<unsigned short>(w0);
+    w0 >>= 16;
+    p += 2;
+  }
+  if (bytes & 1) *p = static_cast<char>(w0);
+}
+// Sixteen elements of a row per lane, `valid` of them and what follows inside the row; prev, next: the
+// lane before, behind holds its neighbours. All lanes of the warp take part. kAny: each lane stores the
+// 16-byte units that start among its elements and end with the next lane's first ones; where there is
+// no such lane, what lies outside whole units is stored in smaller pieces.
+template <typename T, bool kAny>
+SPECB200_DEVINL void store16(T* to, int valid, bool prev, bool next, const Raw16<T>& r) {
+  constexpr int kWords = 4 * sizeof(T), kBytes = 4 * kWords;
+  char* p = reinterpret_cast<char*>(to);
+  int bytes = max(valid, 0) * static_cast<int>(sizeof(T));
+  if constexpr (kAny) {
+    uint32_t w[kWords + 4];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    if constexpr (sizeof(T) == 2) {
-      if (i < valid) reinterpret_cast<unsigned short*>(p)[i] = static_cast<unsigned short>(r.v[i / 2] >> (16 * (i & 1)));
-    } else {
-      if (i < valid) reinterpret_cast<uint32_t*>(p)[i] = r.v[i];
+    for (int i = 0; i < kWords; ++i) w[i] = r.v[i];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[kWords + i] = __shfl_down_sync(0xffffffffu, r.v[i], 1);
+    if (!next) bytes = min(bytes, kBytes);
+    const int head = static_cast<int>(-reinterpret_cast<uintptr_t>(p) & 15);
+    if (!prev && head) {
+      const int n = min(head, bytes);
+#pragma unroll
+      for (int i = 0; i < 16 / static_cast<int>(sizeof(T)); ++i) {
+        if (i * static_cast<int>(sizeof(T)) < n) {
+          if constexpr (sizeof(T) == 2)
+            reinterpret_cast<unsigned short*>(p)[i] = static_cast<unsigned short>(w[i / 2] >> (16 * (i & 1)));
+          else
+            reinterpret_cast<uint32_t*>(p)[i] = w[i];
+        }
+      }
     }
+    shift_words<kWords, sizeof(T) == 2>(w, head);
+#pragma unroll
+    for (int i = 0; i < kWords; i += 4)
+      store_unit(p + head + 4 * i, bytes - head - 4 * i, w[i], w[i + 1], w[i + 2], w[i + 3]);
+  } else {
+    if (valid >= 16) {
+#pragma unroll
+      for (int i = 0; i < kWords; i += 4)
+        *reinterpret_cast<uint4*>(p + 4 * i) = make_uint4(r.v[i], r.v[i + 1], r.v[i + 2], r.v[i + 3]);
+      return;
+    }
+    if (valid <= 0) return;
+#pragma unroll
+    for (int i = 0; i < kWords; i += 4) store_unit(p + 4 * i, bytes - 4 * i, r.v[i], r.v[i + 1], r.v[i + 2], r.v[i + 3]);
   }
 }
 // e4m3(f * inv), 16 of a row, rounded to nearest even. Finite values beyond 448 (a group's maximum can
@@ -144,6 +254,10 @@ SPECB200_DEVINL void store_q16(uint8_t* p, int valid, int align, const f32x2 (&f
   }
   if (align >= 16 && valid >= 16) {
     *reinterpret_cast<uint4*>(p) = make_uint4(v[0], v[1], v[2], v[3]);
+    return;
+  }
+  if (align >= 16) {
+    store_unit(reinterpret_cast<char*>(p), valid, v[0], v[1], v[2], v[3]);
     return;
   }
 #pragma unroll
@@ -191,6 +305,7 @@ struct RowArgs {
   float* scales;       // [M, groups] (or [row blocks, groups])
   int M, K, groups;
   int packed;          // SiLU: 1 = 64 gate columns, then their 64 up columns
+  const void* x_end;   // where x's last row ends
   int vec_in, vec_out; // rows of x / q start on boundaries of this many bytes
 };
 
@@ -198,9 +313,11 @@ constexpr int kRowThreads = 256;
 
 // One group of the row-major list of all groups per 8 lanes, 16 elements each. kSilu: y =
 // silu(gate) * up, else y = x. Bound by memory: what counts is loads in flight, so bf16 keeps to 32
-// registers (8 CTAs per SM); two groups per thread at 48 registers took longer at every size.
-template <typename T, bool kSilu>
-__global__ void __launch_bounds__(kRowThreads, sizeof(T) == 2 ? 8 : 5) quantize_rows_kernel(RowArgs a) {
+// registers (8 CTAs per SM); two groups per thread at 48 registers took longer at every size. SiLU's two
+// inputs off the 16-byte boundaries need more: 16392 x 2047 39.6 us at 6, 43.7 at 8, fp32 56.3 at 4, 60.0 at 5.
+template <typename T, bool kSilu, bool kAny>
+__global__ void __launch_bounds__(kRowThreads, (sizeof(T) == 2 ? 8 : 5) - (kSilu && kAny ? (sizeof(T) == 2 ? 2 : 1) : 0))
+    quantize_rows_kernel(RowArgs a) {
   pdl_launch_dependents();
   const int lane = threadIdx.x & 7;
   const uint32_t groups = a.groups;
@@ -213,22 +330,22 @@ __global__ void __launch_bounds__(kRowThreads, sizeof(T) == 2 ? 8 : 5) quantize_
   const int valid = row < a.M ? a.K - col : 0;
   const T* xr = static_cast<const T*>(a.x) + row * a.ldx;
   pdl_wait();
-  Raw16<T> raw;
+  Loaded16<T, kAny> raw;
   f32x2 y[8];
   if constexpr (kSilu) {
     // packed: feature j is gate column 128 (j / 64) + j % 64, its up column 64 further on
     const int gate = a.packed ? ((col >> 6) << 7) + (col & 63) : col;
-    Raw16<T> raw_up;
-    load16<T>(raw, xr + gate, valid, a.vec_in);
-    load16<T>(raw_up, xr + gate + (a.packed ? 64 : a.K), valid, a.vec_in);
+    Loaded16<T, kAny> raw_up;
+    load16(raw, xr + gate, valid, a.vec_in, a.x, a.x_end);
+    load16(raw_up, xr + gate + (a.packed ? 64 : a.K), valid, a.vec_in, a.x, a.x_end);
     f32x2 up[8];
-    unpack16<T>(raw, y);
-    unpack16<T>(raw_up, up);
+    unpack16<T>(aligned16(raw), y);
+    unpack16<T>(aligned16(raw_up), up);
 #pragma unroll
     for (int j = 0; j < 8; ++j) y[j] = silu_mul2(y[j], up[j]);
   } else {
-    load16<T>(raw, xr + col, valid, a.vec_in);
-    unpack16<T>(raw, y);
+    load16(raw, xr + col, valid, a.vec_in, a.x, a.x_end);
+    unpack16<T>(aligned16(raw), y);
   }
   const float amax = floor_amax(octet_max(max_mag16(y)));
   if (valid > 0) store_q16(a.q + row * a.ldq + col, valid, a.vec_out, y, kE4m3Max / amax);
@@ -236,9 +353,10 @@ __global__ void __launch_bounds__(kRowThreads, sizeof(T) == 2 ? 8 : 5) quantize_
 }
 
 // One 128 x 128 block per CTA, held in registers between the maximum and the rounding: 8 lanes
-// per row, 32 rows at a time.
-template <typename T>
-__global__ void __launch_bounds__(kRowThreads, sizeof(T) == 2 ? 3 : 2) quantize_blocks_kernel(RowArgs a) {
+// per row, 32 rows at a time. Rows off the 16-byte boundaries: a CTA more per SM, although it costs
+// spilled registers (16368 x 2050: 28.3 us, fp32 37.2, against 30.2 and 40.9).
+template <typename T, bool kAny>
+__global__ void __launch_bounds__(kRowThreads, (sizeof(T) == 2 ? 3 : 2) + kAny) quantize_blocks_kernel(RowArgs a) {
   constexpr int kLanes = kRowThreads / 8, kPass = kFp8Group / kLanes;
   __shared__ float sh[kRowThreads / 32];
   pdl_launch_dependents();
@@ -251,15 +369,15 @@ __global__ void __launch_bounds__(kRowThreads, sizeof(T) == 2 ? 3 : 2) quantize_
   const T* xp = static_cast<const T*>(a.x) + first * a.ldx + col;
   uint8_t* qp = a.q + first * a.ldq + col;
   pdl_wait();
-  Raw16<T> x[kPass];
+  Loaded16<T, kAny> x[kPass];
 #pragma unroll
   for (int p = 0; p < kPass; ++p)
-    load16<T>(x[p], xp + p * kLanes * a.ldx, r0 + p * kLanes < rows ? valid : 0, a.vec_in);
+    load16(x[p], xp + p * kLanes * a.ldx, r0 + p * kLanes < rows ? valid : 0, a.vec_in, a.x, a.x_end);
   float m = 0.f;
 #pragma unroll
   for (int p = 0; p < kPass; ++p) {
     f32x2 y[8];
-    unpack16<T>(x[p], y);
+    unpack16<T>(aligned16(x[p]), y);
     m = max_nan(m, max_mag16(y));
   }
 #pragma unroll
@@ -273,7 +391,7 @@ __global__ void __launch_bounds__(kRowThreads, sizeof(T) == 2 ? 3 : 2) quantize_
 #pragma unroll
   for (int p = 0; p < kPass; ++p) {
     f32x2 y[8];
-    unpack16<T>(x[p], y);
+    unpack16<T>(aligned16(x[p]), y);
     if (r0 + p * kLanes < rows && valid > 0) store_q16(qp + p * kLanes * a.ldq, valid, a.vec_out, y, inv);
   }
   if (threadIdx.x == 0) a.scales[blockIdx.x] = amax / kE4m3Max;
@@ -293,6 +411,7 @@ struct NormArgs {
   int M, H, groups;
   int rows;            // rows that a CTA takes at a time
   float eps;
+  const void *x_end, *d_end, *w_end;  // where the last row ends
   int vec_x, vec_d, vec_w, vec_h, vec_q;  // boundaries in bytes
 };
 
@@ -302,9 +421,12 @@ constexpr int kNormMaxWidth = kNormMaxChunks * 64 * kFp8Group;  // 64 octets: 51
 // CTAs per SM that the registers are cut for. 32768 x 2048 bf16 with delta, loads ahead: 71.5 us at 3
 // CTAs (floor 71.9 at the measured copy bandwidth), 81.8 at 2, and 86.2 at 4, which leaves no room for
 // loads ahead; fp32 16384 x 2048: 67.1 at 2, 80.5 at 3. 8192 x 8192 bf16 (two groups per octet): 80.7
-// at 3, 84.4 at 2, 87.4 at 4.
-template <typename T, int kChunks>
-constexpr int kNormCtas = kChunks == 4 ? 1 : kChunks == 2 ? 3 : sizeof(T) == 2 ? 3 : 2;
+// at 3, 84.4 at 2, 87.4 at 4. Rows off the 16-byte boundaries wait longer for more loads, and a few
+// spilled registers cost less than a CTA: 16392 x 2047 bf16 73 us at 4, 91 at 2; fp32 113 at 3, 117 at 2.
+template <typename T, int kChunks, bool kAny>
+constexpr int kNormCtas = kChunks == 4 ? 1
+                                : kAny       ? (sizeof(T) == 2 ? 4 : kChunks == 1 ? 3 : 2)
+                                             : (kChunks == 2 || sizeof(T) == 2 ? 3 : 2);
 
 // h = T(x + delta); y = w h / sqrt(mean(h^2) + eps); (q, scales) = quantize(y).
 //
@@ -317,8 +439,8 @@ constexpr int kNormCtas = kChunks == 4 ? 1 : kChunks == 2 ? 3 : sizeof(T) == 2 ?
 // y / s = (w h r) / (m r / 448) = w h (448 / m), so q carries two roundings and only the scale
 // waits for the row's sum. Where the floor is in play or a value is not finite, q is formed from
 // y itself.
-template <typename T, int kChunks, bool kDelta>
-__global__ void __launch_bounds__(kChunks == 4 ? 512 : 256, kNormCtas<T, kChunks>) rmsnorm_fp8_kernel(NormArgs a) {
+template <typename T, int kChunks, bool kDelta, bool kAny>
+__global__ void __launch_bounds__(kChunks == 4 ? 512 : 256, kNormCtas<T, kChunks, kAny>) rmsnorm_fp8_kernel(NormArgs a) {
   constexpr bool kAhead = kChunks == 1;
   __shared__ float sh[2][64];
   pdl_launch_dependents();
@@ -327,15 +449,19 @@ __global__ void __launch_bounds__(kChunks == 4 ? 512 : 256, kNormCtas<T, kChunks
   const int team = kChunks == 1 ? octet / per_row : 0;
   const int g0 = octet - team * per_row;
   const int col0 = g0 * kFp8Group + (threadIdx.x & 7) * 16;
+  // whether the neighbouring lanes of this warp hold the neighbouring columns
+  const bool prev = (threadIdx.x & 31) != 0 && col0 > 0, next = (threadIdx.x & 31) != 31 && col0 + 16 < per_row * kFp8Group;
   const int pitch = octets * kFp8Group;  // from chunk to chunk of a thread
-  Raw16<T> w[kChunks], x[kChunks], d[kDelta ? kChunks : 1];
+  Raw16<T> w[kChunks];
+  Loaded16<T, kAny> x[kChunks], d[kDelta ? kChunks : 1];
   auto valid_of = [&](int64_t row, int c) { return team < a.rows && row < a.M ? a.H - (col0 + c * pitch) : 0; };
   auto load_row = [&](int64_t row) {
 #pragma unroll
     for (int c = 0; c < kChunks; ++c) {
       const int col = col0 + c * pitch, valid = valid_of(row, c);
-      load16<T>(x[c], static_cast<const T*>(a.x) + row * a.ldx + col, valid, a.vec_x);
-      if constexpr (kDelta) load16<T>(d[c], static_cast<const T*>(a.delta) + row * a.ldd + col, valid, a.vec_d);
+      load16(x[c], static_cast<const T*>(a.x) + row * a.ldx + col, valid, a.vec_x, a.x, a.x_end);
+      if constexpr (kDelta)
+        load16(d[c], static_cast<const T*>(a.delta) + row * a.ldd + col, valid, a.vec_d, a.delta, a.d_end);
     }
   };
   const int64_t step = static_cast<int64_t>(gridDim.x) * a.rows;
@@ -343,8 +469,12 @@ __global__ void __launch_bounds__(kChunks == 4 ? 512 : 256, kNormCtas<T, kChunks
   pdl_wait();
   if constexpr (kAhead) load_row(base + team);
 #pragma unroll
-  for (int c = 0; c < kChunks; ++c)
-    load16<T>(w[c], static_cast<const T*>(a.weight) + col0 + c * pitch, a.H - (col0 + c * pitch), a.vec_w);
+  for (int c = 0; c < kChunks; ++c) {
+    const int col = col0 + c * pitch;
+    Loaded16<T, kAny> l;
+    load16(l, static_cast<const T*>(a.weight) + col, a.H - col, a.vec_w, a.weight, a.w_end);
+    w[c] = aligned16(l);
+  }
   for (int parity = 0; base < a.M; base += step, parity ^= 1) {
     const int64_t row = base + team;
     f32x2 f[kChunks][8];
@@ -352,16 +482,15 @@ __global__ void __launch_bounds__(kChunks == 4 ? 512 : 256, kNormCtas<T, kChunks
     if constexpr (!kAhead) load_row(row);
 #pragma unroll
     for (int c = 0; c < kChunks; ++c) {
-      unpack16<T>(x[c], f[c]);
+      unpack16<T>(aligned16(x[c]), f[c]);
       if constexpr (kDelta) {
         f32x2 g[8];
-        unpack16<T>(d[c], g);
+        unpack16<T>(aligned16(d[c]), g);
 #pragma unroll
         for (int i = 0; i < 8; ++i) f[c][i] = add2(f[c][i], g[i]);
-        x[c] = round16<T>(f[c]);
-        const int col = col0 + c * pitch, valid = valid_of(row, c);
-        if (valid > 0) store16<T>(static_cast<T*>(a.h) + row * a.ldh + col, valid, a.vec_h, x[c]);
-        unpack16<T>(x[c], f[c]);
+        const Raw16<T> h = round16<T>(f[c]);
+        store16<T, kAny>(static_cast<T*>(a.h) + row * a.ldh + col0 + c * pitch, valid_of(row, c), prev, next, h);
+        unpack16<T>(h, f[c]);
       }
     }
     if constexpr (kAhead) {
@@ -432,21 +561,34 @@ unsigned row_ctas(const RowArgs& a) {
   return static_cast<unsigned>((units + per_cta - 1) / per_cta);
 }
 
+// Where the last of M rows of K elements ends.
+template <typename T>
+const void* end_of(const void* x, int64_t ld, int M, int K) {
+  return static_cast<const T*>(x) + (M - 1) * ld + K;
+}
+
+template <typename T, bool kSilu>
+cudaError_t launch_rows(const RowArgs& a, cudaStream_t s) {
+  return a.vec_in >= 16 ? launch_kernel(quantize_rows_kernel<T, kSilu, false>, dim3(row_ctas(a)), dim3(kRowThreads), 0, s, true, a)
+                        : launch_kernel(quantize_rows_kernel<T, kSilu, true>, dim3(row_ctas(a)), dim3(kRowThreads), 0, s, true, a);
+}
+
 template <typename T>
 cudaError_t launch_quantize(RowArgs a, int block_rows, cudaStream_t s) {
   a.vec_in = row_align_of<T>(a.x, a.ldx);
-  if (block_rows == 1) {
-    return launch_kernel(quantize_rows_kernel<T, false>, dim3(row_ctas(a)), dim3(kRowThreads), 0, s, true, a);
-  }
+  a.x_end = end_of<T>(a.x, a.ldx, a.M, a.K);
+  if (block_rows == 1) return launch_rows<T, false>(a, s);
   const unsigned blocks = static_cast<unsigned>(groups_of(a.M)) * a.groups;
-  return launch_kernel(quantize_blocks_kernel<T>, dim3(blocks), dim3(kRowThreads), 0, s, true, a);
+  return a.vec_in >= 16 ? launch_kernel(quantize_blocks_kernel<T, false>, dim3(blocks), dim3(kRowThreads), 0, s, true, a)
+                        : launch_kernel(quantize_blocks_kernel<T, true>, dim3(blocks), dim3(kRowThreads), 0, s, true, a);
 }
 
 template <typename T>
 cudaError_t launch_silu_mul(RowArgs a, cudaStream_t s) {
   a.vec_in = row_align_of<T>(a.x, a.ldx);
+  a.x_end = end_of<T>(a.x, a.ldx, a.M, 2 * a.K);
   if (!a.packed) a.vec_in = std::min(a.vec_in, row_align_of<T>(a.x, a.K));  // where the up columns start
-  return launch_kernel(quantize_rows_kernel<T, true>, dim3(row_ctas(a)), dim3(kRowThreads), 0, s, true, a);
+  return launch_rows<T, true>(a, s);
 }
 
 // As many CTAs as the 148 SMs hold at once, each on every grid-th set of rows. Up to the number that
@@ -461,12 +603,17 @@ cudaError_t launch_filled(K kernel, const NormArgs& a, int threads, cudaStream_t
   }
   return launch_kernel(kernel, dim3(std::min(wanted, 148 * std::max(1, per_sm))), dim3(threads), 0, s, true, a);
 }
+template <typename T, int kChunks, bool kAny>
+cudaError_t launch_norm_rows(const NormArgs& a, int octets, cudaStream_t s) {
+  constexpr int kCtas = kNormCtas<T, kChunks, kAny>;
+  const int threads = (octets * 8 + 31) / 32 * 32;
+  return a.delta ? launch_filled<kCtas>(rmsnorm_fp8_kernel<T, kChunks, true, kAny>, a, threads, s)
+                 : launch_filled<kCtas>(rmsnorm_fp8_kernel<T, kChunks, false, kAny>, a, threads, s);
+}
 template <typename T, int kChunks>
 cudaError_t launch_norm_kernel(const NormArgs& a, int octets, cudaStream_t s) {
-  constexpr int kCtas = kNormCtas<T, kChunks>;
-  const int threads = (octets * 8 + 31) / 32 * 32;
-  return a.delta ? launch_filled<kCtas>(rmsnorm_fp8_kernel<T, kChunks, true>, a, threads, s)
-                 : launch_filled<kCtas>(rmsnorm_fp8_kernel<T, kChunks, false>, a, threads, s);
+  const int align = std::min({a.vec_x, a.vec_d, a.vec_w, a.vec_h});
+  return align >= 16 ? launch_norm_rows<T, kChunks, false>(a, octets, s) : launch_norm_rows<T, kChunks, true>(a, octets, s);
 }
 
 template <typename T>
@@ -475,6 +622,10 @@ cudaError_t launch_rmsnorm_fp8(NormArgs a, cudaStream_t s) {
   a.vec_d = row_align_of<T>(a.delta, a.ldd);
   a.vec_w = row_align(a.weight, 0);
   a.vec_h = row_align_of<T>(a.h, a.ldh);
+  if (!a.delta) a.vec_d = a.vec_h = 32;
+  a.x_end = end_of<T>(a.x, a.ldx, a.M, a.H);
+  a.d_end = a.delta ? end_of<T>(a.delta, a.ldd, a.M, a.H) : nullptr;
+  a.w_end = end_of<T>(a.weight, 0, 1, a.H);
   a.rows = 1;
   if (a.groups > 64) return launch_norm_kernel<T, 4>(a, std::max(32, (a.groups + 3) / 4), s);
   if (a.groups > 32) return launch_norm_kernel<T, 2>(a, (a.groups + 1) / 2, s);

@@ -466,6 +466,63 @@ def test_silu_mul_far_gates():
     assert s.isnan().all() and q.float().isnan().all()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,starts", [(BF16, range(8)), (F32, range(4))])
+@pytest.mark.parametrize("k,pitch", [(301, 301), (5, 5), (130, 134), (2049, 2051), (5002, 5002)])
+def test_rows_on_any_boundary(k, pitch, dtype, starts):
+    """Rows that start anywhere in a 16-byte unit, the first and last ones at the ends of their memory: the
+    same bits as from aligned rows, and the residual stream updated in its place with nothing around it touched."""
+    from specb200 import _ffi
+
+    ops, m = _ops(), 9
+    code, stream = _ffi.BF16 if dtype == BF16 else _ffi.F32, torch.cuda.current_stream().cuda_stream
+    x, d, weight = _rand(13, m, k, dtype=dtype), _rand(14, m, k, dtype=dtype), _rand(15, k, dtype=dtype)
+
+    def aligned(t):
+        held = torch.zeros(t.shape[0], (t.shape[1] + 15) // 16 * 16, dtype=dtype, device=DEV)
+        held[:, :t.shape[1]] = t
+        return held[:, :t.shape[1]]
+
+    def placed(t, start):
+        flat = torch.full(((m - 1) * pitch + k + start,), float("nan"), dtype=dtype, device=DEV)
+        view = flat.as_strided((m, k), (pitch, 1), start)
+        view.copy_(t)
+        return view
+
+    def same(got, want):
+        assert len(got) == len(want)
+        for g, w in zip(got, want):
+            assert torch.equal(g.float(), w.float())
+
+    want_rows, want_blocks = ops.quantize_fp8(aligned(x)), ops.quantize_fp8(aligned(x), block_rows=128)
+    want_norm = ops.rmsnorm_fp8(aligned(x), weight, 1e-5, delta=aligned(d))
+    want_plain = ops.rmsnorm_fp8(aligned(x), weight, 1e-5)
+    assert torch.equal(want_norm[2], (x.float() + d.float()).to(dtype))
+    half = k // 2
+    for start in starts:
+        v = placed(x, start)
+        same(ops.quantize_fp8(v), want_rows)
+        same(ops.quantize_fp8(v, block_rows=128), want_blocks)
+        same(ops.rmsnorm_fp8(v, weight, 1e-5, delta=placed(d, (start * 3) % len(starts))), want_norm)
+        same(ops.rmsnorm_fp8(v, placed(weight[None].expand(m, k), start)[1], 1e-5), want_plain)
+        g, u = v[:, :half].double(), v[:, half:2 * half].double()
+        q, s = ops.silu_mul_fp8(v[:, :2 * half])
+        _check_quantized(q, s, g * torch.sigmoid(g) * u, **_silu_tol(g))
+        # h in x's place inside a frame, through the C ABI
+        frame = torch.full((m * pitch + 40,), 7.0, dtype=dtype, device=DEV)
+        at = 16 + start
+        h = frame.as_strided((m, k), (pitch, 1), at)
+        h.copy_(x)
+        q2, s2 = torch.empty(m, k, dtype=torch.uint8, device=DEV), torch.empty_like(want_norm[1])
+        rc = _lib().specb200_rmsnorm_fp8(code, h.data_ptr(), pitch, d.data_ptr(), k, weight.data_ptr(), m, k, 1e-5,
+                                         h.data_ptr(), pitch, q2.data_ptr(), k, s2.data_ptr(), stream)
+        assert rc == 0
+        same((q2.view(F8), s2, h), want_norm)
+        outside = torch.ones_like(frame, dtype=torch.bool)
+        outside.as_strided((m, k), (pitch, 1), at).fill_(False)
+        assert (frame[outside] == 7).all()
+
+
 # ---------------------------------------------------------------- linear
 LINEAR = [(1, 1, 1), (1, 16, 16), (1, 128, 128), (2, 130, 129), (5, 960, 576), (8, 256, 2048), (9, 6144, 2048),
           (33, 2048, 8192), (16, 500, 4096), (17, 500, 4096), (15, 40000, 256), (64, 1000, 1000), (127, 300, 200), (128, 128, 640), (129, 257, 384), (320, 2048, 1024),
