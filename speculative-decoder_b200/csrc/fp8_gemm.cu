@@ -298,7 +298,9 @@ SPECB200_DEVINL void store_warp_tile(const F8Args& a, const CUtensorMap& y_map, 
     }
     for (int c = c0; c < c0 + kRound; c += kPiece) {
       if (by_tma(c)) continue;
-      // a row at a time, four bytes per lane: one element, or the pair that starts on a 4-byte boundary
+      // A row at a time, four bytes per lane: one element, or the pair that starts on a 4-byte boundary.
+      // 4096 x 8190 x 64: 39 us (an element per store 123, eight bytes per lane with the rows' ends in
+      // smaller pieces 42, fp32 49 and 57).
       const int rows = min(32, a.M - m0), left = a.N - n0 - c;
       const uint8_t* piece = bufs + (c - c0) / kPiece * kF8OutPiece + (lane & 3) * 4;
       T* y = static_cast<T*>(a.y) + static_cast<int64_t>(m0) * a.ldy + n0 + c;

@@ -112,9 +112,15 @@ Quantized quantized_like(const at::Tensor& x, int64_t k, at::IntArrayRef scale_s
   Quantized out;
   out.pitch = padded(k);
   c10::SmallVector<int64_t, 6> sizes(x.sizes().begin(), x.sizes().end());
-  sizes.back() = out.pitch;
-  out.q = empty_beside(x, sizes, at::kFloat8_e4m3fn);
-  if (out.pitch != k) out.q = out.q.narrow(-1, 0, k);
+  sizes.back() = k;
+  if (out.pitch == k) {
+    out.q = empty_beside(x, sizes, at::kFloat8_e4m3fn);
+  } else {
+    c10::SmallVector<int64_t, 6> strides(sizes.size(), 1);
+    int64_t stride = out.pitch;
+    for (size_t d = sizes.size() - 1; d-- > 0; stride *= sizes[d]) strides[d] = stride;
+    out.q = at::Tensor(at::detail::empty_strided_cuda(sizes, strides, at::kFloat8_e4m3fn, x.device()));
+  }
   sizes.back() = groups_of(k);
   out.scales = empty_beside(x, scale_sizes.empty() ? at::IntArrayRef(sizes) : scale_sizes, at::kFloat);
   return out;
