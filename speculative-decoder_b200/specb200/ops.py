@@ -173,7 +173,8 @@ def quantize_fp8(x: torch.Tensor, block_rows: int = 1) -> tuple[torch.Tensor, to
     """e4m3 values and fp32 scales of x [..., K]: s = max(max |x|, 2^-100) / 448 over each group,
     q = e4m3(x / s). block_rows 1 (activations): a scale per row and 128 columns,
     [..., ceil(K / 128)]. block_rows 128 (weights, x [N, K]): one per 128 x 128 block,
-    [ceil(N / 128), ceil(K / 128)]. q's rows are padded to 16 bytes in memory."""
+    [ceil(N / 128), ceil(K / 128)]. q's rows, like those of all the 8-bit operators' outputs, start on
+    16-byte boundaries: where K is not a multiple of 16, q has a row stride beyond K."""
     return _ext().quantize_fp8(x, block_rows)
 
 
@@ -181,7 +182,8 @@ def rmsnorm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float,
                 delta: torch.Tensor | None = None) -> tuple[torch.Tensor, ...]:
     """RMSNorm with an 8-bit output: (q, scales) of weight * h / sqrt(mean(h^2) + eps) for h = x
     [..., H], the values of quantize_fp8 on the fp32 product. With delta, the residual update
-    h = x + delta (rounded to x's dtype) comes first and the result is (q, scales, h)."""
+    h = x + delta (rounded to x's dtype) comes first and the result is (q, scales, h), h's rows on
+    16-byte boundaries as q's."""
     return _ext().rmsnorm_fp8(x, weight, eps, delta)
 
 
@@ -196,6 +198,7 @@ def linear_fp8(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scale
     """x [..., K] @ w[N, K]^T on e4m3 operands with a scale per 128 of K (quantize_fp8, rmsnorm_fp8,
     silu_mul_fp8: x_scales [..., ceil(K / 128)]) and per 128 x 128 block of w (quantize_fp8 with
     block_rows 128: w_scales [ceil(N / 128), ceil(K / 128)]); fp32 accumulation, bf16 or fp32 out.
-    Operands whose rows are not on 16-byte boundaries are copied there first. check reads the device
-    status back (and waits for the stream)."""
+    Operands whose rows are not on 16-byte boundaries are copied there first; the output's rows start on
+    them (a row stride beyond N where N is odd). check reads the device status back (and waits for the
+    stream, so a call that is captured into a graph has check=False)."""
     return _ext().linear_fp8(x, x_scales, w, w_scales, out_f32, check)

@@ -556,6 +556,30 @@ def test_linear_of_views():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("k,n", [(300, 1001), (256, 640), (77, 3)])
+def test_outputs_start_on_16_byte_boundaries(k, n):
+    """Rows of every output start on them, dense where their length allows it; leading dimensions merge as
+    those of a dense tensor, and each output is the next call's input as it is."""
+    ops = _ops()
+    x, d = _rand(16, 2, 3, k, dtype=BF16), _rand(17, 2, 3, k, dtype=BF16)
+    q, s, h = ops.rmsnorm_fp8(x, _rand(18, k, dtype=BF16), 1e-5, delta=d)
+    w, ws = ops.quantize_fp8(_rand(19, n, k, dtype=BF16), block_rows=128)
+    y = ops.linear_fp8(q, s, w, ws)
+    y32 = ops.linear_fp8(q, s, w, ws, out_f32=True)
+    for t in (q, h, w, y, y32):
+        assert t.stride(-1) == 1 and (t.stride(-2) * t.element_size()) % 16 == 0 and t.data_ptr() % 16 == 0
+        assert t.is_contiguous() == (t.shape[-1] * t.element_size() % 16 == 0)
+    for t in (q, h, y, y32):
+        assert t.view(6, t.shape[-1]).stride(0) == t.stride(1) and t.stride(0) == 3 * t.stride(1)
+    assert torch.equal(h, (x.float() + d.float()).bfloat16())
+    _check_product(y.view(6, n), q.view(6, k), s.view(6, -1), w, ws, False)
+    _check_product(y32.view(6, n), q.view(6, k), s.view(6, -1), w, ws, True)
+    again = ops.quantize_fp8(y)
+    dense = ops.quantize_fp8(y.contiguous())
+    assert torch.equal(again[0].float(), dense[0].float()) and torch.equal(again[1], dense[1])
+
+
+@pytest.mark.gpu
 def test_linear_output_pitch_and_frame():
     """Through the C ABI: an output with a pitch of its own (odd: scalar stores) keeps what lies around it."""
     lib = _lib()
