@@ -271,7 +271,9 @@ int specb200_attention(int dtype, const void* q, const void* k_pool, const void*
  * Activations [M, K] have a scale per row and 128 columns: scales [M, ceil(K / 128)] fp32.
  * Weights [N, K] have one per 128 x 128 block: [ceil(N / 128), ceil(K / 128)]. The last groups
  * may be short. Row pitches (ld*) count elements; any pitch and alignment is accepted except
- * where a function says otherwise, rows on 16-byte boundaries are faster. A NaN in a group
+ * where a function says otherwise, rows on 16-byte boundaries are faster (from others whole 16-byte
+ * units are read, so what lies between two rows may be read, but nothing before the first row or
+ * behind the last). A NaN in a group
  * makes its values and scale NaN, an infinity makes the scale infinite. Nothing is written
  * behind a row's last element. Outputs must not overlap inputs unless a function says so.
  * M = 0 is a no-op. No workspaces: calls on any streams may overlap.
@@ -282,7 +284,7 @@ int specb200_quantize_fp8(int dtype, const void* x, int64_t ldx, int M, int K, i
                           int64_t ldq, float* scales, void* stream);
 
 /* RMSNorm with the residual update in front and an 8-bit output:
- *   h = T(x + delta) (delta NULL: h = x, not stored; h may be x or delta),
+ *   h = T(x + delta) (delta NULL: h = x, not stored; h may be x or delta, with its pitch),
  *   y = weight * h / sqrt(mean(h^2) + eps) in fp32, (q, scales) = quantized y.
  * H <= 32768 (SPECB200_ERR_UNSUPPORTED beyond). */
 int specb200_rmsnorm_fp8(int dtype, const void* x, int64_t ldx, const void* delta, int64_t ldd, const void* weight,
