@@ -52,7 +52,7 @@ struct Raw16 {
 // The same as they are loaded. kAny = false: rows start on 16-byte boundaries; one or two 256-bit
 // loads (or 128-bit ones, align 16). kAny = true: rows start anywhere, and what is loaded is the
 // 16-byte units that the elements lie in, `shift` bytes of the first one ahead of them (16384 x 2050
-// bf16: quantize 23.7 us, RMSNorm 90; with a load per element 38 and 207).
+// bf16: quantize 23.7 us, RMSNorm 79; with a load per element 38 and 207).
 template <typename T, bool kAny>
 struct Loaded16 {
   uint32_t v[4 * sizeof(T) + (kAny ? 4 : 0)];
@@ -421,18 +421,18 @@ constexpr int kNormMaxWidth = kNormMaxChunks * 64 * kFp8Group;  // 64 octets: 51
 // CTAs per SM that the registers are cut for. 32768 x 2048 bf16 with delta, loads ahead: 71.5 us at 3
 // CTAs (floor 71.9 at the measured copy bandwidth), 81.8 at 2, and 86.2 at 4, which leaves no room for
 // loads ahead; fp32 16384 x 2048: 67.1 at 2, 80.5 at 3. 8192 x 8192 bf16 (two groups per octet): 80.7
-// at 3, 84.4 at 2, 87.4 at 4. Rows off the 16-byte boundaries wait longer for more loads, and a few
-// spilled registers cost less than a CTA: 16392 x 2047 bf16 73 us at 4, 91 at 2; fp32 113 at 3, 117 at 2.
+// at 3, 84.4 at 2, 87.4 at 4. Rows off the 16-byte boundaries need their registers for the units and
+// hide the loads behind other CTAs' work: 16392 x 2047 bf16 63 us at 4, 72 with loads ahead; fp32 92 and 113.
 template <typename T, int kChunks, bool kAny>
 constexpr int kNormCtas = kChunks == 4 ? 1
-                                : kAny       ? (sizeof(T) == 2 ? 4 : kChunks == 1 ? 3 : 2)
+                                : kAny       ? (kChunks == 2 && sizeof(T) == 4 ? 2 : 4)
                                              : (kChunks == 2 || sizeof(T) == 2 ? 3 : 2);
 
 // h = T(x + delta); y = w h / sqrt(mean(h^2) + eps); (q, scales) = quantize(y).
 //
 // Eight lanes hold one group of a row (kChunks groups of a wide one); a CTA takes as many rows at
 // a time as it has octets for, and walks over the rows with its weights in registers. With one group per
-// octet the next rows' loads are issued before the current rows' sums are formed. A row's sum of squares is added
+// octet and rows on 16-byte boundaries the next rows' loads are issued before the current rows' sums are formed. A row's sum of squares is added
 // within each octet by shuffles, then over the octets in a fixed order.
 //
 // The quantized values need no norm: with m the group's largest |w h| and r the row's 1 / rms,
@@ -441,7 +441,7 @@ constexpr int kNormCtas = kChunks == 4 ? 1
 // y itself.
 template <typename T, int kChunks, bool kDelta, bool kAny>
 __global__ void __launch_bounds__(kChunks == 4 ? 512 : 256, kNormCtas<T, kChunks, kAny>) rmsnorm_fp8_kernel(NormArgs a) {
-  constexpr bool kAhead = kChunks == 1;
+  constexpr bool kAhead = kChunks == 1 && !kAny;
   __shared__ float sh[2][64];
   pdl_launch_dependents();
   const int octet = threadIdx.x >> 3, octets = blockDim.x >> 3;
