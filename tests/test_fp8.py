@@ -668,6 +668,41 @@ def test_offsets_past_32_bits():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", [(3, 2048, 2048), (16, 19200, 256), (60, 1024, 2048), (300, 9000, 256)])
+def test_weights_written_by_the_kernel_in_front(m, n, k):
+    """One weight buffer, quantized anew right in front of each product, eagerly and in a graph: a kernel that
+    starts early must not see what lay there before."""
+    from specb200 import _ffi
+
+    ops, lib = _ops(), _lib()
+    x, xs = ops.quantize_fp8(_rand(90, m, k, dtype=BF16))
+    source = [_rand(91 + i, n, k, dtype=BF16) for i in range(3)]
+    want = [ops.linear_fp8(x, xs, *ops.quantize_fp8(w, block_rows=128)) for w in source]
+    w, ws = ops.quantize_fp8(source[0], block_rows=128)
+    got = torch.zeros(12, m, n, dtype=BF16, device=DEV)
+
+    def run():
+        stream = torch.cuda.current_stream().cuda_stream
+        for i in range(12):
+            rc = lib.specb200_quantize_fp8(_ffi.BF16, source[i % 3].data_ptr(), k, n, k, 128, w.data_ptr(), k,
+                                           ws.data_ptr(), stream)
+            assert rc == 0
+            rc = lib.specb200_linear_fp8(x.data_ptr(), x.stride(0), xs.data_ptr(), w.data_ptr(), k, ws.data_ptr(), m, n, k,
+                                         0, got[i].data_ptr(), n, None, stream)
+            assert rc == 0
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run()
+    for call in (run, graph.replay, graph.replay):
+        got.zero_()
+        call()
+        torch.cuda.synchronize()
+        for i in range(12):
+            assert torch.equal(got[i], want[i % 3])
+
+
+@pytest.mark.gpu
 def test_capture_with_a_status_word():
     """Through the C ABI, whose call clears the status word in front of the kernel."""
     lib = _lib()
