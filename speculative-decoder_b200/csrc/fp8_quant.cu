@@ -52,7 +52,8 @@ struct Raw16 {
 // The same as they are loaded. kAny = false: rows start on 16-byte boundaries; one or two 256-bit
 // loads (or 128-bit ones, align 16). kAny = true: rows start anywhere, and what is loaded is the
 // 16-byte units that the elements lie in, `shift` bytes of the first one ahead of them (16384 x 2050
-// bf16: quantize 23.7 us, RMSNorm 79; with a load per element 38 and 207).
+// bf16: quantize 22.7 us, RMSNorm 72; with a load per element 38 and 207; with 32-byte units, fewer loads and
+// more to shift, 25.6 and 84).
 template <typename T, bool kAny>
 struct Loaded16 {
   uint32_t v[4 * sizeof(T) + (kAny ? 4 : 0)];
@@ -116,19 +117,34 @@ SPECB200_DEVINL void load16(Loaded16<T, kAny>& r, const T* p, int valid, int ali
     }
   }
 }
-// w[0..kOut) = the words that start `bytes` (0..15, even) into w.
-template <int kOut, bool kHalves>
+// w[0..kOut) = the words that start `bytes` (0..15, even) into w. kJump: a jump to code for each number of
+// words instead of selects, the same one for a whole row. It pays where one or two shifts stand in a
+// kernel of few registers (16392 x 2047 bf16: RMSNorm 59 us against 63, rows quantized 20.3 and 21.7) and
+// not for blocks (31.7 and 28.7, fp32 56 and 38), SiLU (fp32 58.6 and 56.2) or the fp32 norm (93 and 92).
+template <int kOut, bool kHalves, int kSkip>
+SPECB200_DEVINL void shift_from(uint32_t (&w)[kOut + 4], uint32_t bits) {
+#pragma unroll
+  for (int i = 0; i < kOut; ++i) w[i] = kHalves ? __funnelshift_r(w[i + kSkip], w[i + kSkip + (kHalves ? 1 : 0)], bits) : w[i + kSkip];
+}
+template <int kOut, bool kHalves, bool kJump>
 SPECB200_DEVINL void shift_words(uint32_t (&w)[kOut + 4], uint32_t bytes) {
+  const uint32_t bits = (bytes & 2) * 8;
+  if constexpr (kJump) {
+    switch (bytes >> 2) {
+      case 0: shift_from<kOut, kHalves, 0>(w, bits); break;
+      case 1: shift_from<kOut, kHalves, 1>(w, bits); break;
+      case 2: shift_from<kOut, kHalves, 2>(w, bits); break;
+      default: shift_from<kOut, kHalves, 3>(w, bits); break;
+    }
+  } else {
 #pragma unroll
-  for (int i = 0; i < kOut + 2; ++i) w[i] = bytes & 8 ? w[i + 2] : w[i];
+    for (int i = 0; i < kOut + 2; ++i) w[i] = bytes & 8 ? w[i + 2] : w[i];
 #pragma unroll
-  for (int i = 0; i < kOut + 1; ++i) w[i] = bytes & 4 ? w[i + 1] : w[i];
-  if constexpr (kHalves) {
-#pragma unroll
-    for (int i = 0; i < kOut; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], (bytes & 2) * 8);
+    for (int i = 0; i < kOut + 1; ++i) w[i] = bytes & 4 ? w[i + 1] : w[i];
+    if constexpr (kHalves) shift_from<kOut, kHalves, 0>(w, bits);
   }
 }
-template <typename T, bool kAny>
+template <bool kJump, typename T, bool kAny>
 SPECB200_DEVINL Raw16<T> aligned16(const Loaded16<T, kAny>& l) {
   constexpr int kWords = 4 * sizeof(T);
   Raw16<T> r;
@@ -136,7 +152,7 @@ SPECB200_DEVINL Raw16<T> aligned16(const Loaded16<T, kAny>& l) {
     uint32_t w[kWords + 4];
 #pragma unroll
     for (int i = 0; i < kWords + 4; ++i) w[i] = l.v[i];
-    shift_words<kWords, sizeof(T) == 2>(w, l.shift);
+    shift_words<kWords, sizeof(T) == 2, kJump>(w, l.shift);
 #pragma unroll
     for (int i = 0; i < kWords; ++i) r.v[i] = w[i];
   } else {
@@ -225,7 +241,7 @@ SPECB200_DEVINL void store16(T* to, int valid, bool prev, bool next, const Raw16
         }
       }
     }
-    shift_words<kWords, sizeof(T) == 2>(w, head);
+    shift_words<kWords, sizeof(T) == 2, sizeof(T) == 2>(w, head);
 #pragma unroll
     for (int i = 0; i < kWords; i += 4)
       store_unit(p + head + 4 * i, bytes - head - 4 * i, w[i], w[i + 1], w[i + 2], w[i + 3]);
@@ -339,13 +355,13 @@ __global__ void __launch_bounds__(kRowThreads, (sizeof(T) == 2 ? 8 : 5) - (kSilu
     load16(raw, xr + gate, valid, a.vec_in, a.x, a.x_end);
     load16(raw_up, xr + gate + (a.packed ? 64 : a.K), valid, a.vec_in, a.x, a.x_end);
     f32x2 up[8];
-    unpack16<T>(aligned16(raw), y);
-    unpack16<T>(aligned16(raw_up), up);
+    unpack16<T>(aligned16<false>(raw), y);
+    unpack16<T>(aligned16<false>(raw_up), up);
 #pragma unroll
     for (int j = 0; j < 8; ++j) y[j] = silu_mul2(y[j], up[j]);
   } else {
     load16(raw, xr + col, valid, a.vec_in, a.x, a.x_end);
-    unpack16<T>(aligned16(raw), y);
+    unpack16<T>(aligned16<true>(raw), y);
   }
   const float amax = floor_amax(octet_max(max_mag16(y)));
   if (valid > 0) store_q16(a.q + row * a.ldq + col, valid, a.vec_out, y, kE4m3Max / amax);
@@ -377,7 +393,7 @@ __global__ void __launch_bounds__(kRowThreads, (sizeof(T) == 2 ? 3 : 2) + kAny) 
 #pragma unroll
   for (int p = 0; p < kPass; ++p) {
     f32x2 y[8];
-    unpack16<T>(aligned16(x[p]), y);
+    unpack16<T>(aligned16<false>(x[p]), y);
     m = max_nan(m, max_mag16(y));
   }
 #pragma unroll
@@ -391,7 +407,7 @@ __global__ void __launch_bounds__(kRowThreads, (sizeof(T) == 2 ? 3 : 2) + kAny) 
 #pragma unroll
   for (int p = 0; p < kPass; ++p) {
     f32x2 y[8];
-    unpack16<T>(aligned16(x[p]), y);
+    unpack16<T>(aligned16<false>(x[p]), y);
     if (r0 + p * kLanes < rows && valid > 0) store_q16(qp + p * kLanes * a.ldq, valid, a.vec_out, y, inv);
   }
   if (threadIdx.x == 0) a.scales[blockIdx.x] = amax / kE4m3Max;
@@ -422,7 +438,8 @@ constexpr int kNormMaxWidth = kNormMaxChunks * 64 * kFp8Group;  // 64 octets: 51
 // CTAs (floor 71.9 at the measured copy bandwidth), 81.8 at 2, and 86.2 at 4, which leaves no room for
 // loads ahead; fp32 16384 x 2048: 67.1 at 2, 80.5 at 3. 8192 x 8192 bf16 (two groups per octet): 80.7
 // at 3, 84.4 at 2, 87.4 at 4. Rows off the 16-byte boundaries need their registers for the units and
-// hide the loads behind other CTAs' work: 16392 x 2047 bf16 63 us at 4, 72 with loads ahead; fp32 92 and 113.
+// hide the loads behind other CTAs' work: 16392 x 2047 bf16 59 us, fp32 92 (63 and 92 against 72 and 113 with loads
+// ahead, before the last step).
 template <typename T, int kChunks, bool kAny>
 constexpr int kNormCtas = kChunks == 4 ? 1
                                 : kAny       ? (kChunks == 2 && sizeof(T) == 4 ? 2 : 4)
@@ -441,7 +458,7 @@ constexpr int kNormCtas = kChunks == 4 ? 1
 // y itself.
 template <typename T, int kChunks, bool kDelta, bool kAny>
 __global__ void __launch_bounds__(kChunks == 4 ? 512 : 256, kNormCtas<T, kChunks, kAny>) rmsnorm_fp8_kernel(NormArgs a) {
-  constexpr bool kAhead = kChunks == 1 && !kAny;
+  constexpr bool kAhead = kChunks == 1 && !kAny, kJump = sizeof(T) == 2;
   __shared__ float sh[2][64];
   pdl_launch_dependents();
   const int octet = threadIdx.x >> 3, octets = blockDim.x >> 3;
@@ -473,7 +490,7 @@ __global__ void __launch_bounds__(kChunks == 4 ? 512 : 256, kNormCtas<T, kChunks
     const int col = col0 + c * pitch;
     Loaded16<T, kAny> l;
     load16(l, static_cast<const T*>(a.weight) + col, a.H - col, a.vec_w, a.weight, a.w_end);
-    w[c] = aligned16(l);
+    w[c] = aligned16<false>(l);
   }
   for (int parity = 0; base < a.M; base += step, parity ^= 1) {
     const int64_t row = base + team;
@@ -482,10 +499,10 @@ __global__ void __launch_bounds__(kChunks == 4 ? 512 : 256, kNormCtas<T, kChunks
     if constexpr (!kAhead) load_row(row);
 #pragma unroll
     for (int c = 0; c < kChunks; ++c) {
-      unpack16<T>(aligned16(x[c]), f[c]);
+      unpack16<T>(aligned16<kJump>(x[c]), f[c]);
       if constexpr (kDelta) {
         f32x2 g[8];
-        unpack16<T>(aligned16(d[c]), g);
+        unpack16<T>(aligned16<kJump>(d[c]), g);
 #pragma unroll
         for (int i = 0; i < 8; ++i) f[c][i] = add2(f[c][i], g[i]);
         const Raw16<T> h = round16<T>(f[c]);
