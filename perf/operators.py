@@ -196,18 +196,13 @@ def _engine(state):
                           out_f32=case["dtype"] == "f32", check=False)
 
 
-_loaded = []
-
-
 def _ops():
-    if not _loaded:  # imported once, as a program does
-        package = str(Path.cwd() / "speculative-decoder_b200")
-        if package not in sys.path:
-            sys.path.insert(0, package)
-        from specb200 import ops
+    package = str(Path.cwd() / "speculative-decoder_b200")
+    if package not in sys.path:
+        sys.path.insert(0, package)
+    from specb200 import ops
 
-        _loaded.append(ops)
-    return _loaded[0]
+    return ops
 
 
 def _split_gate_up(gate_up, packed):
