@@ -279,7 +279,10 @@ int specb200_attention(int dtype, const void* q, const void* k_pool, const void*
  * M = 0 is a no-op. No workspaces: calls on any streams may overlap.
  * ====================================================================================== */
 
-/* block_rows 1: a scale per row and 128 columns; 128: per 128 x 128 block. x: [M, K] of `dtype`. */
+/* block_rows 1: a scale per row and 128 columns; 128: per 128 x 128 block. x: [M, K] of `dtype`. s is the fp32
+ * quotient and q that of x / s with the stored s, rounded to fp32 before e4m3 (for fp32 one x / s in 2^18
+ * may be an fp32 ulp off, for maxima beyond 2^110 one in 2^6). The fused forms below leave up to 4 fp32
+ * half steps in y / s, as well as what their y carries. */
 int specb200_quantize_fp8(int dtype, const void* x, int64_t ldx, int M, int K, int block_rows, void* q,
                           int64_t ldq, float* scales, void* stream);
 

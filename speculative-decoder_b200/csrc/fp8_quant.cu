@@ -257,15 +257,14 @@ SPECB200_DEVINL void store16(T* to, int valid, bool prev, bool next, const Raw16
     for (int i = 0; i < kWords; i += 4) store_unit(p + 4 * i, bytes - 4 * i, r.v[i], r.v[i + 1], r.v[i + 2], r.v[i + 3]);
   }
 }
-// e4m3(f * inv), 16 of a row, rounded to nearest even. Finite values beyond 448 (a group's maximum can
+// e4m3 of 16 values of a row, rounded to nearest even. Finite values beyond 448 (a group's maximum can
 // exceed it by an ulp) saturate, NaN stays NaN.
-SPECB200_DEVINL void store_q16(uint8_t* p, int valid, int align, const f32x2 (&f)[8], float inv) {
-  const f32x2 inv2 = pack2(inv, inv);
+SPECB200_DEVINL void store_e4m3_16(uint8_t* p, int valid, int align, const f32x2 (&f)[8]) {
   uint32_t v[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint32_t lo = __nv_cvt_float2_to_fp8x2(unpack2(mul2(f[2 * i], inv2)), __NV_SATFINITE, __NV_E4M3);
-    const uint32_t hi = __nv_cvt_float2_to_fp8x2(unpack2(mul2(f[2 * i + 1], inv2)), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(unpack2(f[2 * i]), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(unpack2(f[2 * i + 1]), __NV_SATFINITE, __NV_E4M3);
     v[i] = lo | (hi << 16);
   }
   if (align >= 16 && valid >= 16) {
@@ -279,6 +278,52 @@ SPECB200_DEVINL void store_q16(uint8_t* p, int valid, int align, const f32x2 (&f
 #pragma unroll
   for (int i = 0; i < 16; ++i)
     if (i < valid) p[i] = static_cast<uint8_t>(v[i / 4] >> (8 * (i & 3)));
+}
+
+// e4m3(f * inv).
+SPECB200_DEVINL void store_q16(uint8_t* p, int valid, int align, const f32x2 (&f)[8], float inv) {
+  const f32x2 inv2 = pack2(inv, inv);
+  f32x2 t[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) t[i] = mul2(f[i], inv2);
+  store_e4m3_16(p, valid, align, t);
+}
+
+// A group's scale, and what divides by it. Where elements lie between two e4m3 numbers the quotient often
+// does so too but for the scale's own rounding (bf16 ones most of all), so q = e4m3(x / s) is formed from
+// the IEEE quotient by the scale as it is stored: whoever holds x and s can form the same q. Products with
+// 448 / amax put up to 0.2 % of a weight matrix on the other side.
+//
+// The scale: amax (hi + lo) with hi + lo = 1 / 448 to 2^-51 and one rounding of the sum. amax / 7 lies at
+// least 1/14 ulp from the middle of two fp32 numbers, so this is the IEEE quotient.
+// Elements: 1 / s as hi + lo, hi below it and lo > 0, so that zeros keep their signs. x hi + x lo is off by less
+// than 2^-42 of itself before its one rounding (the reciprocal by at most 2^-22, which lo corrects). No
+// pair of bf16 mantissas puts x / s within 2^-40 of the middle of two fp32 numbers (the test looks at them
+// all), so this is the IEEE quotient; for fp32 one quotient in 2^18 is next to such a middle and may go
+// an ulp the other way, which e4m3 sees where it is next to the middle of two of its numbers as well.
+// Maxima beyond 2^110 leave lo in the subnormal range and x hi + x lo off by up to 2^-30 before the rounding.
+// quantize 32768 x 2048 bf16: 31.5 us (32.0 by products and IEEE divisions for s and 448 / amax, 37.4 with a
+// division's correction step instead of lo); weight blocks 16384 x 2048 18.4 (17.6).
+struct Divisor {
+  float s;       // the scale
+  float hi, lo;  // 1 / s
+};
+SPECB200_DEVINL Divisor divisor_of(float amax) {
+  Divisor c;
+  const bool finite = amax <= 3.402823466e38f;  // else q = x * (1 / s), which is 0 or NaN
+  c.s = finite ? fmaf(amax, 0x1.24924ap-9f, amax * -0x1.b6db6ep-34f) : amax;
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(c.s));
+  c.hi = r * (1.f - 0x1p-21f);
+  c.lo = finite ? fmaf(-c.s, c.hi, 1.f) * r : 0.f;
+  return c;
+}
+// e4m3(f / c.s).
+SPECB200_DEVINL void store_quotients16(uint8_t* p, int valid, int align, f32x2 (&f)[8], const Divisor& c) {
+  const f32x2 hi = pack2(c.hi, c.hi), lo = pack2(c.lo, c.lo);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = fma2(f[i], hi, mul2(f[i], lo));
+  store_e4m3_16(p, valid, align, f);
 }
 
 SPECB200_DEVINL float max_mag16(const f32x2 (&f)[8]) {
@@ -364,13 +409,20 @@ __global__ void __launch_bounds__(kRowThreads, (sizeof(T) == 2 ? 8 : 5) - (kSilu
     unpack16<T>(aligned16<true>(raw), y);
   }
   const float amax = floor_amax(octet_max(max_mag16(y)));
-  if (valid > 0) store_q16(a.q + row * a.ldq + col, valid, a.vec_out, y, kE4m3Max / amax);
-  if (row < a.M && lane == 0) a.scales[row * groups + g] = amax / kE4m3Max;
+  if constexpr (kSilu) {
+    if (valid > 0) store_q16(a.q + row * a.ldq + col, valid, a.vec_out, y, kE4m3Max / amax);
+    if (row < a.M && lane == 0) a.scales[row * groups + g] = amax / kE4m3Max;
+  } else {
+    const Divisor c = divisor_of(amax);
+    if (valid > 0) store_quotients16(a.q + row * a.ldq + col, valid, a.vec_out, y, c);
+    if (row < a.M && lane == 0) a.scales[row * groups + g] = c.s;
+  }
 }
 
 // One 128 x 128 block per CTA, held in registers between the maximum and the rounding: 8 lanes
 // per row, 32 rows at a time. Rows off the 16-byte boundaries: a CTA more per SM, although it costs
-// spilled registers (16368 x 2050: 28.3 us, fp32 37.2, against 30.2 and 40.9).
+// spilled registers (16368 x 2050: 29.9 us, fp32 40.8; before the quotients by the stored scale 28.3 and
+// 37.2, against 30.2 and 40.9 with a CTA less).
 template <typename T, bool kAny>
 __global__ void __launch_bounds__(kRowThreads, (sizeof(T) == 2 ? 3 : 2) + kAny) quantize_blocks_kernel(RowArgs a) {
   constexpr int kLanes = kRowThreads / 8, kPass = kFp8Group / kLanes;
@@ -402,15 +454,14 @@ __global__ void __launch_bounds__(kRowThreads, (sizeof(T) == 2 ? 3 : 2) + kAny) 
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < kRowThreads / 32; ++i) m = max_nan(m, sh[i]);
-  const float amax = floor_amax(m);
-  const float inv = kE4m3Max / amax;
+  const Divisor c = divisor_of(floor_amax(m));
 #pragma unroll
   for (int p = 0; p < kPass; ++p) {
     f32x2 y[8];
     unpack16<T>(aligned16<false>(x[p]), y);
-    if (r0 + p * kLanes < rows && valid > 0) store_q16(qp + p * kLanes * a.ldq, valid, a.vec_out, y, inv);
+    if (r0 + p * kLanes < rows && valid > 0) store_quotients16(qp + p * kLanes * a.ldq, valid, a.vec_out, y, c);
   }
-  if (threadIdx.x == 0) a.scales[blockIdx.x] = amax / kE4m3Max;
+  if (threadIdx.x == 0) a.scales[blockIdx.x] = c.s;
 }
 
 struct NormArgs {

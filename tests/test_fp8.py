@@ -13,6 +13,7 @@ Tolerances, with u = 2^-24 (half a step of fp32):
 from __future__ import annotations
 
 import ctypes
+from fractions import Fraction
 
 import pytest
 import torch
@@ -261,6 +262,68 @@ def test_quantize_edge_values(block_rows):
     rest = qi[rows_i].clone()
     rest[rows_i.index(1), 0] = 0
     assert (rest == 0).all()
+
+
+def _fp32(v):
+    """The fp32 number nearest to a positive fraction, ties to even, and half a step there (no underflow)."""
+    e = v.numerator.bit_length() - v.denominator.bit_length()
+    if Fraction(2) ** e > v:
+        e -= 1
+    step = Fraction(2) ** (e - 23)
+    return round(v / step) * step, step / 2
+
+
+def test_quotients_of_bf16_values_keep_off_the_middle_of_two_fp32_numbers():
+    """x / s with s = amax / 448 rounded to fp32, over all bf16 mantissas of x and amax (powers of two change
+    nothing): whatever is within 2^-41 of the quotient, relatively, rounds as the quotient does. The bf16
+    quantizer forms it to 2^-42 before the rounding."""
+    for amax in range(128, 256):
+        s, _ = _fp32(Fraction(amax, 448))
+        for x in range(128, 256):
+            quotient = x / s
+            nearest, half = _fp32(quotient)
+            assert half - abs(quotient - nearest) > quotient * Fraction(1, 2 ** 41), (x, amax)
+
+
+def test_scales_are_quotients_by_448():
+    """amax hi + amax lo with hi + lo = 1 / 448 to 2^-51: amax / 448 is no nearer than 2^-28 of itself to the
+    middle of two fp32 numbers, because the distance is a multiple of 1 / 14 of a step."""
+    for amax in list(range(2 ** 23, 2 ** 24, 9973)) + list(range(2 ** 24 - 64, 2 ** 24)):
+        quotient = Fraction(amax, 448)
+        nearest, half = _fp32(quotient)
+        assert half - abs(quotient - nearest) >= half / 7 > quotient * Fraction(1, 2 ** 28)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("block_rows", [1, 128])
+@pytest.mark.parametrize("m,k,start", [(321, 2048, 0), (300, 1000, 0), (130, 301, 3), (1, 127, 1)])
+def test_quantize_divides_by_the_scale_it_returns(m, k, start, block_rows, dtype):
+    """Bit for bit s = max(max |x|, 2^-100) / 448 and q = e4m3(x / s) in fp32, from rows on 16-byte boundaries and
+    off them: ordinary values, whole numbers (whose quotients lie between two e4m3 numbers but for the
+    scale's rounding), columns below the floor and beyond 1e30, zeros of both signs, a NaN and an infinity."""
+    wide = _rand(m + k, m, k + start, dtype=dtype)
+    whole = torch.randint(-300, 301, (m, k + start), generator=torch.Generator().manual_seed(m)).to(DEV, dtype)
+    far = wide.clone()
+    for i, factor in enumerate((1e-38, 1e-33, 2.0 ** -64, 1e-12, 1e12, 2.0 ** 60, 1e30)):
+        far[:, 128 * i:128 * (i + 1)] *= factor
+    far[:, ::5] = 0
+    far[:, 2::10] = -0.0
+    odd = wide.clone()
+    odd[m // 2, k // 2] = float("nan")
+    odd[m // 3, 0] = float("-inf")
+    for held in (wide, whole, far, odd):
+        x = held[:, start:]
+        q, s = _ops().quantize_fp8(x, block_rows=block_rows)
+        f = torch.nn.functional.pad(x.float().abs(), (0, -k % 128, 0, -m % block_rows))
+        # in 64 bits, then rounded: torch multiplies fp32 CUDA tensors by 1 / 448 where it is asked to divide by a number
+        want = (f.reshape(f.shape[0] // block_rows, block_rows, -1, 128).amax(dim=(1, 3)).clamp_min(FLOOR).double() / 448).float()
+        assert torch.equal(s.view(torch.int32)[~s.isnan()], want.view(torch.int32)[~want.isnan()])
+        assert torch.equal(s.isnan(), want.isnan())
+        quotient = (x.float() / _spread(want, m, k, block_rows)).to(F8)
+        nan = quotient.float().isnan()
+        assert torch.equal(q.float().isnan(), nan)
+        assert torch.equal(q.contiguous().view(torch.uint8)[~nan], quotient.view(torch.uint8)[~nan])
 
 
 @pytest.mark.gpu
