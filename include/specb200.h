@@ -281,8 +281,8 @@ int specb200_attention(int dtype, const void* q, const void* k_pool, const void*
 
 /* block_rows 1: a scale per row and 128 columns; 128: per 128 x 128 block. x: [M, K] of `dtype`. s is the fp32
  * quotient and q that of x / s with the stored s, rounded to fp32 before e4m3 (for fp32 one x / s in 2^18
- * may be an fp32 ulp off, for maxima beyond 2^110 one in 2^6). The fused forms below leave up to 4 fp32
- * half steps in y / s, as well as what their y carries. */
+ * may be an fp32 ulp off, for maxima beyond 2^110 one in 2^6). SiLU does
+ * the same with its fp32 y; RMSNorm, whose y / s needs no 1 / rms, leaves up to 4 fp32 half steps in it. */
 int specb200_quantize_fp8(int dtype, const void* x, int64_t ldx, int M, int K, int block_rows, void* q,
                           int64_t ldq, float* scales, void* stream);
 

@@ -342,10 +342,9 @@ SPECB200_DEVINL float octet_max(float m) {
   return m;
 }
 
-// silu(g) * u = g u / (1 + 2^(-g log2 e)) for a pair. The exponent is rounded to fp32, which leaves
+// silu(g) * u = g u / (1 + 2^(-g log2 e)) for a pair, g >= -87. The exponent is rounded to fp32, which leaves
 // |g| 2^-23 in the exponential: nothing next to the 1 for positive gates, and for negative ones a
-// relative error that grows as the value itself dies away. Where the exponential overflows its
-// reciprocal is zero; an infinite gate gives what the formula gives (inf u, or NaN).
+// relative error that grows as the value itself dies away. An infinite gate gives inf u.
 SPECB200_DEVINL f32x2 silu_mul2(f32x2 g, f32x2 u) {
   constexpr float kLog2e = 1.44269504f;
   const float2 t = unpack2(mul2(g, pack2(-kLog2e, -kLog2e)));
@@ -356,6 +355,30 @@ SPECB200_DEVINL f32x2 silu_mul2(f32x2 g, f32x2 u) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s.x) : "f"(d.x));
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s.y) : "f"(d.y));
   return mul2(mul2(g, pack2(s.x, s.y)), u);
+}
+
+// The same below -87, where the 1 is nothing next to the exponential and the exponential's reciprocal leaves
+// fp32's range (the fast reciprocal is zero from -87.34 on): e^g in two halves, one for each factor, which
+// reaches as far down as any fp32 `up` can lift the value above what e4m3 holds (-177). -inf gives NaN, as
+// the formula does.
+SPECB200_DEVINL float silu_mul_far(float g, float u) {
+  const float half = expf(0.5f * g);
+  return (g * half) * (half * u);
+}
+// Whether any of 16 gates is below -87 (or a NaN with a sign): as whole numbers, these are the ones above
+// that of -87.
+template <typename T>
+SPECB200_DEVINL bool any_far(const Raw16<T>& g) {
+  uint32_t m = g.v[0];
+  if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int i = 1; i < 8; ++i) m = __vmaxu2(m, g.v[i]);
+    return max(m >> 16, m & 0xffffu) > 0xc2aeu;
+  } else {
+#pragma unroll
+    for (int i = 1; i < 16; ++i) m = max(m, g.v[i]);
+    return m > 0xc2ae0000u;
+  }
 }
 
 struct RowArgs {
@@ -375,7 +398,7 @@ constexpr int kRowThreads = 256;
 // One group of the row-major list of all groups per 8 lanes, 16 elements each. kSilu: y =
 // silu(gate) * up, else y = x. Bound by memory: what counts is loads in flight, so bf16 keeps to 32
 // registers (8 CTAs per SM); two groups per thread at 48 registers took longer at every size. SiLU's two
-// inputs off the 16-byte boundaries need more: 16392 x 2047 39.6 us at 6, 43.7 at 8, fp32 56.3 at 4, 60.0 at 5.
+// inputs off the 16-byte boundaries need more: 16392 x 2047 39.6 us at 6, 43.7 at 8, fp32 56.3 at 4, 60.0 at 5 (now 40.0 and 56.6).
 template <typename T, bool kSilu, bool kAny>
 __global__ void __launch_bounds__(kRowThreads, (sizeof(T) == 2 ? 8 : 5) - (kSilu && kAny ? (sizeof(T) == 2 ? 2 : 1) : 0))
     quantize_rows_kernel(RowArgs a) {
@@ -400,23 +423,32 @@ __global__ void __launch_bounds__(kRowThreads, (sizeof(T) == 2 ? 8 : 5) - (kSilu
     load16(raw, xr + gate, valid, a.vec_in, a.x, a.x_end);
     load16(raw_up, xr + gate + (a.packed ? 64 : a.K), valid, a.vec_in, a.x, a.x_end);
     f32x2 up[8];
-    unpack16<T>(aligned16<false>(raw), y);
+    const Raw16<T> gates = aligned16<false>(raw);
+    unpack16<T>(gates, y);
     unpack16<T>(aligned16<false>(raw_up), up);
+    const bool far = any_far(gates);
 #pragma unroll
     for (int j = 0; j < 8; ++j) y[j] = silu_mul2(y[j], up[j]);
+    if (far) {  // rare: the elements are read again, so that the registers of the others need not be kept
+      const T* gp = xr + gate;
+      const T* upp = gp + (a.packed ? 64 : a.K);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        float2 v = unpack2(y[j]);
+        const float g0 = 2 * j < valid ? to_f32(gp[2 * j]) : 0.f, g1 = 2 * j + 1 < valid ? to_f32(gp[2 * j + 1]) : 0.f;
+        if (g0 < -87.f) v.x = silu_mul_far(g0, to_f32(upp[2 * j]));
+        if (g1 < -87.f) v.y = silu_mul_far(g1, to_f32(upp[2 * j + 1]));
+        y[j] = pack2(v.x, v.y);
+      }
+    }
   } else {
     load16(raw, xr + col, valid, a.vec_in, a.x, a.x_end);
     unpack16<T>(aligned16<true>(raw), y);
   }
   const float amax = floor_amax(octet_max(max_mag16(y)));
-  if constexpr (kSilu) {
-    if (valid > 0) store_q16(a.q + row * a.ldq + col, valid, a.vec_out, y, kE4m3Max / amax);
-    if (row < a.M && lane == 0) a.scales[row * groups + g] = amax / kE4m3Max;
-  } else {
-    const Divisor c = divisor_of(amax);
-    if (valid > 0) store_quotients16(a.q + row * a.ldq + col, valid, a.vec_out, y, c);
-    if (row < a.M && lane == 0) a.scales[row * groups + g] = c.s;
-  }
+  const Divisor c = divisor_of(amax);
+  if (valid > 0) store_quotients16(a.q + row * a.ldq + col, valid, a.vec_out, y, c);
+  if (row < a.M && lane == 0) a.scales[row * groups + g] = c.s;
 }
 
 // One 128 x 128 block per CTA, held in registers between the maximum and the rounding: 8 lanes

@@ -529,6 +529,42 @@ def test_silu_mul_far_gates():
     assert s.isnan().all() and q.float().isnan().all()
 
 
+# Below -87: e^(g/2) to 4 u (2 ulp) twice, four products and the half steps of the fp32 gate and up themselves, which
+# are exact; subnormal halves (below -174.7) keep at least 20 bits down to -177. 16 u with those, 2^-18.
+def _check_far(x, k, packed=False):
+    q, s = _ops().silu_mul_fp8(x, packed=packed)
+    g, u = x.view(x.shape[0], k // 64, 2, 64).unbind(2) if packed else (x[:, :k], x[:, k:])
+    g, u = g.reshape(-1, k).double(), u.reshape(-1, k).double()
+    y = g * u / (1 + torch.exp(-g))
+    far = 2 * U * g.abs().max().item() + 16 * U if (g > -87).any() else 16 * U
+    far = max(far, 2.0 ** -18) if (g < -174).any() else far
+    _check_quantized(q, s, y, d=2 * far + 2 * U, s_tol=far + 2 * U)
+    return q
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("packed", [False, True])
+def test_silu_mul_gates_whose_sigmoid_leaves_fp32(dtype, packed):
+    """Groups that hold nothing but far gates, with `up` values large enough to lift them above the floor: around
+    -87 .. -89, where a rounded-off reciprocal is zero first, and on to where no fp32 `up` lifts them."""
+    k = 1024
+    for lo, hi, up in ((-88.7, -87.36, 1e8), (-90.0, -85.0, 1e12), (-104.0, -80.0, 1e20), (-150.0, -100.0, 1e37),
+                       (-176.0, -150.0, 3e38), (-177.0, -60.0, 1e37)):
+        g = torch.linspace(lo, hi, 3 * k, device=DEV).view(3, k)
+        u = up * (1 - 0.3 * torch.rand(3, k, generator=torch.Generator().manual_seed(3)).to(DEV))
+        x = torch.stack([v.view(3, k // 64, 64) for v in (g, u)], 2).reshape(3, 2 * k) if packed else torch.cat([g, u], 1)
+        q = _check_far(x.to(dtype).contiguous(), k, packed)
+        assert (q.float() != 0).any(), (lo, hi)
+    # gates beyond any range, and the formula's values for infinite ones
+    g = torch.full((1, 128), -1e4, device=DEV)
+    q, s = _ops().silu_mul_fp8(torch.cat([g, torch.full_like(g, 3e38)], 1).to(dtype))
+    assert (q.float() == 0).all() and (s == FLOOR / 448).all()
+    g[0, 3] = float("-inf")
+    q, s = _ops().silu_mul_fp8(torch.cat([g, torch.full_like(g, 2.0)], 1).to(dtype))
+    assert s.isnan().all()
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype,starts", [(BF16, range(8)), (F32, range(4))])
 @pytest.mark.parametrize("k,pitch", [(301, 301), (5, 5), (130, 134), (2049, 2051), (5002, 5002)])
