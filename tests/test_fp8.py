@@ -802,6 +802,25 @@ def test_weights_written_by_the_kernel_in_front(m, n, k):
 
 
 @pytest.mark.gpu
+def test_a_long_chain_of_products():
+    """Products of the longest K back to back, each 0.44 s on one cluster: later ones start beside the earlier ones, and
+    the time for which they wait for those (more than a wait's limit of 2 s) is no reason to give up."""
+    lib = _lib()
+    k = 2 ** 30
+    x = torch.zeros(1, k, dtype=torch.uint8, device=DEV)
+    x[0, torch.randperm(k // 1024, generator=torch.Generator().manual_seed(1))[:1000].to(DEV) * 1024 + 77] = 0x38  # 1.0
+    w = torch.full((1, k), 0x38, dtype=torch.uint8, device=DEV)
+    scales = torch.ones(1, k // 128, device=DEV)
+    y = torch.full((9, 4), -7.0, device=DEV)
+    stream = torch.cuda.current_stream().cuda_stream
+    for row in y:
+        rc = lib.specb200_linear_fp8(x.data_ptr(), k, scales.data_ptr(), w.data_ptr(), k, scales.data_ptr(), 1, 1, k, 1,
+                                     row.data_ptr(), 4, None, stream)
+        assert rc == 0
+    assert (y[:, 0] == 1000).all() and (y[:, 1:] == -7).all()
+
+
+@pytest.mark.gpu
 def test_capture_with_a_status_word():
     """Through the C ABI, whose call clears the status word in front of the kernel."""
     lib = _lib()
