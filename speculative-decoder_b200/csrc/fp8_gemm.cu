@@ -481,16 +481,15 @@ __global__ void __launch_bounds__(f8_small_threads(kPerSm), kPerSm)
     }
     __syncwarp();
     asm volatile("cp.async.wait_all;" ::: "memory");
-    pdl_launch_dependents();
   } else if (warp == 9) {
     f8_tmem_alloc<false>(&bars.tmem_holder, kBufs * kF8Block);
     tc_fence_before();
     __syncwarp();
     tc_fence_after();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&bars.tmem_holder);
-    // Only from here on may the next kernel's CTAs start (each warp allows it once it knows of the
-    // allocation): one that allocated TMEM before this CTA and then waited for it would keep it
-    // from ever starting.
+    // Only from here on may the next kernel's CTAs start: one that allocated TMEM before this CTA and then
+    // waited for it would keep it from ever starting. The first thread that allows it does so for the
+    // whole CTA, so no other warp does.
     pdl_launch_dependents();
     constexpr uint32_t idesc = umma_idesc_e4m3(kF8TileM, kF8Block);
     const uint32_t leader = elect_leader();
@@ -533,7 +532,6 @@ __global__ void __launch_bounds__(f8_small_threads(kPerSm), kPerSm)
     auto factor = [&] { return scales[slot].x[quarter * 32 + lane] * scales[slot].w[0]; };
     bool ok = ready(try_ready());
     const uint32_t tbase = ok ? *reinterpret_cast<volatile uint32_t*>(&bars.tmem_holder) + (static_cast<uint32_t>(quarter * 32) << 16) + col0 : 0;
-    pdl_launch_dependents();
     int groups = kb1 - kb0;
     if (!live) {
       while (ok) {
@@ -718,7 +716,6 @@ __global__ void __launch_bounds__(kF8FewThreads, 2)
     }
     __syncwarp();
     asm volatile("cp.async.wait_all;" ::: "memory");
-    pdl_launch_dependents();
   } else if (warp == 9) {
     f8_tmem_alloc<false>(&bars.tmem_holder, kBufs * kTok);
     tc_fence_before();
@@ -750,10 +747,7 @@ __global__ void __launch_bounds__(kF8FewThreads, 2)
       ok = wait_warp<true>(&done[st], phase, &sfull[slot], slot_phase, a.status, &abort_flag);
       if (!ok) break;
       tc_fence_after();
-      if (g == odd) {
-        tbase = *reinterpret_cast<volatile uint32_t*>(&bars.tmem_holder) + (static_cast<uint32_t>(quarter * 32) << 16);
-        pdl_launch_dependents();
-      }
+      if (g == odd) tbase = *reinterpret_cast<volatile uint32_t*>(&bars.tmem_holder) + (static_cast<uint32_t>(quarter * 32) << 16);
       const F8Scales& sc = scales[slot];
       const float w = sc.w[0];
       uint32_t r[kTok];

@@ -821,6 +821,48 @@ def test_a_long_chain_of_products():
 
 
 @pytest.mark.gpu
+def test_kernels_that_hold_tensor_memory_take_turns():
+    """Short products of every kind (all of their groups fit the rings) and bf16 ones back to back in changing orders,
+    eagerly and in a graph: whichever starts beside which, each gets its accumulators and its result."""
+    from specb200 import _ffi
+
+    ops, lib = _ops(), _lib()
+    shapes = [(5, 2048, 512), (16, 25600, 128), (100, 900, 384), (64, 25600, 256), (300, 9000, 256), (3, 2048, 2048)]
+    held = [_operands(70 + i, *s) for i, s in enumerate(shapes)]
+    want = [ops.linear_fp8(*h) for h in held]
+    x, w = _rand(71, 40, 512, dtype=BF16), _rand(72, 4096, 512, dtype=BF16)
+    want.append(ops.linear(x, w))
+    ws = torch.empty(max(16, lib.specb200_linear_workspace_bytes(40, 4096, 512)), dtype=torch.uint8, device=DEV)
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    orders = [torch.randperm(7, generator=torch.Generator().manual_seed(i)).tolist() for i in range(8)]
+
+    def run():
+        out = []
+        for i in (i for order in orders for i in order):
+            if i < 6:
+                out.append((i, ops.linear_fp8(*held[i], check=False)))
+                continue
+            y = torch.empty_like(want[6])
+            rc = lib.specb200_linear(_ffi.BF16, w.data_ptr(), x.data_ptr(), 40, 4096, 512, 0, y.data_ptr(), ws.data_ptr(),
+                                     ws.numel(), status.data_ptr(), torch.cuda.current_stream().cuda_stream)
+            assert rc == 0
+            out.append((i, y))
+        return out
+
+    for i, y in run():
+        assert torch.equal(y, want[i]), shapes[i] if i < 6 else "bf16"
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    for i, y in out:
+        assert torch.equal(y, want[i])
+    assert int(status) == 0
+
+
+@pytest.mark.gpu
 def test_capture_with_a_status_word():
     """Through the C ABI, whose call clears the status word in front of the kernel."""
     lib = _lib()
