@@ -303,10 +303,18 @@ int specb200_silu_mul_fp8(int dtype, const void* gate_up, int64_t ld, int M, int
 /* y[m, n] = sum_b x_scales[m, b] * w_scales[n / 128, b] * sum_{k in group b} x[m, k] * w[n, k] on
  * the tensor cores, accumulated in fp32. x [M, K], w [N, K] e4m3: bases on 16-byte boundaries,
  * pitches multiples of 16. y: fp32 (out_f32) or bf16. Results do not depend on scheduling.
- * status: device int32, or NULL; cleared by the call, set if a device-side wait gave up. */
+ * status: device int32, or NULL; cleared by the call, set if a device-side wait gave up. What such a wait
+ * leaves unfinished is written as NaN, with or without a status word. */
 int specb200_linear_fp8(const void* x, int64_t ldx, const float* x_scales, const void* w, int64_t ldw,
                         const float* w_scales, int M, int N, int K, int out_f32, void* y, int64_t ldy,
                         int32_t* status, void* stream);
+
+/* The failure path of linear_fp8's waits, like specb200_wait_probe: the same call and the same kernels, but no
+ * operand is ever loaded, so after about two seconds every wait for one gives up with nothing in
+ * flight, y is NaN and status (if given) SPECB200_ERR_TIMEOUT. */
+int specb200_linear_fp8_wait_probe(const void* x, int64_t ldx, const float* x_scales, const void* w, int64_t ldw,
+                                   const float* w_scales, int M, int N, int K, int out_f32, void* y, int64_t ldy,
+                                   int32_t* status, void* stream);
 
 #ifdef __cplusplus
 }

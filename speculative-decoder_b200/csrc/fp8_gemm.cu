@@ -59,6 +59,7 @@ struct F8Args {
   int out_f32;
   int rows16;           // y's rows are on 16-byte boundaries: tiles are written by TMA, split ones in quads
   int tail16;           // ... and end on one
+  int starved;          // no operand is ever loaded: every wait for one runs out
   int32_t* status;
 };
 
@@ -275,6 +276,23 @@ SPECB200_DEVINL void tma_store_2d(const CUtensorMap* map, const void* smem_src, 
                : "memory");
 }
 
+// NaN for what a warp could not finish because a wait gave up, so that the caller sees it without a status word
+// too: up to 32 tokens of its features, and in a cluster's partial tile what the splits add up. (NaN in the
+// sums on the way of the ordinary stores cost every call of the small kernel 0.15 us.)
+constexpr uint32_t kF8Nan = 0x7fffffffu;
+SPECB200_DEVINL void give_up_outputs(const F8Args& a, int m0, int n0, int cols, int lane) {
+  const int rows = min(32, a.M - m0), end = min(n0 + cols, a.N);
+  for (int r = 0; r < rows; ++r) {
+    const int64_t at = static_cast<int64_t>(m0 + r) * a.ldy;
+    for (int n = n0 + lane; n < end; n += 32) {
+      if (a.out_f32)
+        static_cast<uint32_t*>(a.y)[at + n] = kF8Nan;
+      else
+        static_cast<unsigned short*>(a.y)[at + n] = static_cast<unsigned short>(kF8Nan >> 16);
+    }
+  }
+}
+
 // One warp's 32 tokens x kCols features to memory through kPieces pieces of shared memory, a piece
 // being 128 bytes per row (64 bf16 or 32 fp32 features). The 16-byte units of a row are swizzled by
 // the row (the 128-byte swizzle TMA reads), so that neither side has bank conflicts. TMA stores
@@ -443,7 +461,7 @@ __global__ void __launch_bounds__(f8_small_threads(kPerSm), kPerSm)
     const float* sx = a.xs + static_cast<int64_t>(tile_m + lane) * a.kblocks + kb0;
     const float* sw = a.ws + static_cast<int64_t>(tile_n / kF8Block) * a.kblocks + kb0;
     const int64_t pitch32 = static_cast<int64_t>(32) * a.kblocks;
-    const int tokens = a.M - tile_m, groups = kb1 - kb0, me = warp == 8 ? 0 : 1;
+    const int tokens = a.M - tile_m, groups = a.starved ? 0 : kb1 - kb0, me = warp == 8 ? 0 : 1;
     auto load = [&](int g, uint32_t st) {
       if (lane == 0) {
         uint8_t* s = smem + st * stage_bytes;
@@ -602,14 +620,18 @@ __global__ void __launch_bounds__(f8_small_threads(kPerSm), kPerSm)
       } else {
         store_warp_tile<__nv_bfloat16, 1>(a, y_map, acc, smem + warp * kF8OutPiece, m0, n0, lane);
       }
+    } else if (live && splits > 1) {
+      for (int i = 0; i < kCols && m0 + lane < a.M; ++i)
+        reinterpret_cast<uint32_t*>(smem)[(quarter * 32 + lane) * kPitch + col0 + i] = kF8Nan;
+    } else if (live) {
+      give_up_outputs(a, m0, n0, kCols, lane);
     }
     if (a.rows16 && splits == 1 && lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
   }
   __syncwarp();
   if (splits > 1) {
     cluster_arrive_wait();
-    if (!*reinterpret_cast<volatile int*>(&abort_flag))
-      add_split_tiles(a, smem_u32(smem), tile_m, tile_n, min(kF8TileM, a.M - tile_m), split, kThreads);
+    add_split_tiles(a, smem_u32(smem), tile_m, tile_n, min(kF8TileM, a.M - tile_m), split, kThreads);
     cluster_arrive_wait();  // no CTA leaves while another reads its shared memory
   }
   tc_fence_before();
@@ -696,11 +718,11 @@ __global__ void __launch_bounds__(kF8FewThreads, 2)
       copy_async_arrive(&sfull[slot]);
     };
     // as in the small kernel
-    const int first = min(groups, static_cast<int>(stages));
+    const int loads = a.starved ? 0 : groups, first = min(loads, static_cast<int>(stages));
     for (int g = me; g < first; g += kProducers) load(g, g);
     for (int g = me; g < first; g += kProducers) fetch(g, g);
     uint32_t st = 0, phase = 0, slot = stages;
-    for (int g = first; g < groups; ++g) {
+    for (int g = first; g < loads; ++g) {
       if (g % kProducers == me) {
         if (!wait_warp(&done[st], phase, a.status, &abort_flag)) {
           for (int i = max(0, g - static_cast<int>(stages)); i < g; ++i)
@@ -769,6 +791,10 @@ __global__ void __launch_bounds__(kF8FewThreads, 2)
       if (slot >= stages + kBufs) { slot -= stages + kBufs; slot_phase ^= 1; }
       buf ^= 2;
     }
+    if (!ok) {
+#pragma unroll
+      for (int i = 0; i < kTok; ++i) acc[i] = __uint_as_float(kF8Nan);
+    }
     // the odd groups' sums to shared memory, the even groups' added to them
     if (odd) {
 #pragma unroll
@@ -776,7 +802,7 @@ __global__ void __launch_bounds__(kF8FewThreads, 2)
         if (i < a.M) sums[i * kPitch + feature] = acc[i];
     }
     asm volatile("bar.sync 1, 256;" ::: "memory");
-    if (!odd && ok) {
+    if (!odd) {
       const int n = tile_n + feature;
 #pragma unroll
       for (int i = 0; i < kTok; ++i) {
@@ -794,7 +820,7 @@ __global__ void __launch_bounds__(kF8FewThreads, 2)
   __syncwarp();
   if (splits > 1) {
     cluster_arrive_wait();
-    if (!*reinterpret_cast<volatile int*>(&abort_flag)) add_split_tiles(a, smem_u32(sums), 0, tile_n, a.M, split, kF8FewThreads);
+    add_split_tiles(a, smem_u32(sums), 0, tile_n, a.M, split, kF8FewThreads);
     cluster_arrive_wait();  // no CTA leaves while another reads its shared memory
   }
   tc_fence_before();
@@ -909,7 +935,7 @@ __global__ void __launch_bounds__(kF8PairThreads, 1)
         const float* sw = a.ws + static_cast<int64_t>(block) * kblocks;
         const bool live_w = lane < 2 && block * kF8Block < a.N;
         for (int kb = 0; kb < kblocks; ++kb, mine = !mine) {
-          if (mine) {
+          if (mine && !a.starved) {
             ok = wait_warp(&bars.done[1][st], phase ^ 1, a.status, &abort_flag);
             if (!ok) break;
             if (lane == 0) {
@@ -993,7 +1019,8 @@ __global__ void __launch_bounds__(kF8PairThreads, 1)
       return __all_sync(0xffffffffu, tried) || wait_warp(&bars.done[1][st], phase, a.status, &abort_flag);
     };
     auto factor = [&] { return bars.scales[slot].x[quarter * 32 + lane] * bars.scales[slot].w[block]; };
-    for (F8TileWalk tile(a); tile.more() && ok; tile.next()) {
+    F8TileWalk tile(a);
+    for (; tile.more() && ok; tile.next()) {
       const int m0 = tile.token0(rank) + quarter * 32, n0 = tile.feature0() + block * kF8Block;
       if (m0 >= a.M || n0 >= a.N) {  // a warp without outputs only keeps step
         for (int kb = 0; kb < kblocks; ++kb) {
@@ -1058,6 +1085,8 @@ __global__ void __launch_bounds__(kF8PairThreads, 1)
       else
         store_warp_tile<__nv_bfloat16, kF8PairPieces>(a, y_map, acc, out_buf, m0, n0, lane);
     }
+    for (; tile.more() && !ok; tile.next())
+      give_up_outputs(a, tile.token0(rank) + quarter * 32, tile.feature0() + block * kF8Block, kCols, lane);
     if (a.rows16 && lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
     __syncwarp();
   }
@@ -1180,9 +1209,9 @@ cudaError_t launch_fp8(const F8Plan& p, const CUtensorMap& wm, const CUtensorMap
 using namespace specb200;
 extern "C" int specb200_set_error(int code, const char* msg);
 
-extern "C" int specb200_linear_fp8(const void* x, int64_t ldx, const float* x_scales, const void* w, int64_t ldw,
-                                   const float* w_scales, int M, int N, int K, int out_f32, void* y, int64_t ldy,
-                                   int32_t* status, void* stream) {
+namespace {
+int run_linear_fp8(const void* x, int64_t ldx, const float* x_scales, const void* w, int64_t ldw, const float* w_scales,
+                   int M, int N, int K, int out_f32, void* y, int64_t ldy, bool starved, int32_t* status, void* stream) {
   if (M < 0 || N <= 0 || K <= 0 || M > (1 << 30) || N > (1 << 30) || K > (1 << 30))
     return specb200_set_error(SPECB200_ERR_ARG, "linear_fp8: bad M/N/K");
   if (ldx < K || ldw < K || ldx % 16 || ldw % 16 || ldy < N)
@@ -1223,9 +1252,23 @@ extern "C" int specb200_linear_fp8(const void* x, int64_t ldx, const float* x_sc
   a.out_f32 = out_f32 ? 1 : 0;
   a.rows16 = y_rows16;
   a.tail16 = (static_cast<int64_t>(N) * esize) % 16 == 0;
+  a.starved = starved;
   a.status = status;
   cudaError_t e = cudaSuccess;
   if (status) e = cudaMemsetAsync(status, 0, sizeof(int32_t), s);
   if (e == cudaSuccess) e = launch_fp8(p, wm, xm, ym, a, s);
   return e == cudaSuccess ? SPECB200_OK : specb200_set_error(SPECB200_ERR_CUDA, cudaGetErrorString(e));
+}
+}  // namespace
+
+extern "C" int specb200_linear_fp8(const void* x, int64_t ldx, const float* x_scales, const void* w, int64_t ldw,
+                                   const float* w_scales, int M, int N, int K, int out_f32, void* y, int64_t ldy,
+                                   int32_t* status, void* stream) {
+  return run_linear_fp8(x, ldx, x_scales, w, ldw, w_scales, M, N, K, out_f32, y, ldy, false, status, stream);
+}
+
+extern "C" int specb200_linear_fp8_wait_probe(const void* x, int64_t ldx, const float* x_scales, const void* w, int64_t ldw,
+                                              const float* w_scales, int M, int N, int K, int out_f32, void* y, int64_t ldy,
+                                              int32_t* status, void* stream) {
+  return run_linear_fp8(x, ldx, x_scales, w, ldw, w_scales, M, N, K, out_f32, y, ldy, true, status, stream);
 }

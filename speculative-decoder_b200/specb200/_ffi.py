@@ -90,6 +90,8 @@ PROTOTYPES: dict[str, tuple] = {
                                       c_void_p]),
     "specb200_linear_fp8": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int, c_int, c_int,
                                     c_int, c_void_p, c_int64, c_void_p, c_void_p]),
+    "specb200_linear_fp8_wait_probe": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int, c_int,
+                                               c_int, c_int, c_void_p, c_int64, c_void_p, c_void_p]),
 }
 
 _lib: ctypes.CDLL | None = None

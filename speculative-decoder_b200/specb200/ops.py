@@ -200,5 +200,6 @@ def linear_fp8(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scale
     block_rows 128: w_scales [ceil(N / 128), ceil(K / 128)]); fp32 accumulation, bf16 or fp32 out.
     Operands whose rows are not on 16-byte boundaries are copied there first; the output's rows start on
     them (a row stride beyond N where N is odd). check reads the device status back (and waits for the
-    stream, so a call that is captured into a graph has check=False)."""
+    stream, so a call that is captured into a graph has check=False). Without it nothing is raised for a
+    device-side wait that gave up; what it left unfinished is NaN either way."""
     return _ext().linear_fp8(x, x_scales, w, w_scales, out_f32, check)

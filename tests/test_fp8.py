@@ -802,6 +802,30 @@ def test_weights_written_by_the_kernel_in_front(m, n, k):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k,f32,with_status", [
+    (5, 200, 256, 1, True), (3, 300, 2048, 0, False), (16, 19000, 128, 0, True), (40, 200, 256, 0, True),
+    (40, 333, 4096, 1, False), (20, 19100, 128, 0, True), (300, 9001, 256, 0, True), (2000, 5000, 128, 1, False)])
+def test_linear_whose_waits_run_out(m, n, k, f32, with_status):
+    """Every kind of product (few tokens, single, split and shared SMs, pairs over one and three tiles) without any
+    operand: each wait gives up by itself, all outputs are NaN whether or not a status word is given, nothing
+    around them is touched, and the next call is right."""
+    from specb200 import _ffi
+
+    ops, lib = _ops(), _lib()
+    x, xs, w, ws = _operands(5, m, n, k)
+    y = torch.full((m + 2, n + 3), 9.0, dtype=F32 if f32 else BF16, device=DEV)
+    status = torch.full((1,), 77, dtype=torch.int32, device=DEV)
+    rc = lib.specb200_linear_fp8_wait_probe(x.data_ptr(), x.stride(0), xs.data_ptr(), w.data_ptr(), w.stride(0), ws.data_ptr(),
+                                            m, n, k, f32, y[1].data_ptr(), n + 3, status.data_ptr() if with_status else None,
+                                            torch.cuda.current_stream().cuda_stream)
+    assert rc == 0
+    assert y[1:-1, :n].isnan().all()
+    assert (y[0] == 9).all() and (y[-1] == 9).all() and (y[:, n:] == 9).all()
+    assert int(status) == (_ffi.ERR_TIMEOUT if with_status else 77)
+    _check_product(ops.linear_fp8(x, xs, w, ws, out_f32=bool(f32)), x, xs, w, ws, bool(f32))
+
+
+@pytest.mark.gpu
 def test_a_long_chain_of_products():
     """Products of the longest K back to back, each 0.44 s on one cluster: later ones start beside the earlier ones, and
     the time for which they wait for those (more than a wait's limit of 2 s) is no reason to give up."""
