@@ -326,4 +326,9 @@ PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_torch_ops", nullptr, -1, meth
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__torch_ops() { return PyModule_Create(&module_def); }
+// `target`: what the module was compiled for, which specb200/_ffi.py compares with what runs.
+PyMODINIT_FUNC PyInit__torch_ops() {
+  PyObject* m = PyModule_Create(&module_def);
+  if (m && PyModule_AddStringConstant(m, "target", SPECB200_TARGET) < 0) Py_CLEAR(m);
+  return m;
+}

@@ -114,12 +114,17 @@ def lib() -> ctypes.CDLL:
 
 
 def torch_ops():
-    """The extension module specb200._torch_ops. Raises if it has not been built."""
+    """The extension module specb200._torch_ops. Raises if it has not been built for this torch and Python."""
     try:
         from specb200 import _torch_ops
     except ImportError as e:
         raise RuntimeError(f"specb200/_torch_ops.so cannot be loaded ({e}): build it with `python -m specb200.build` "
                            "(the engine has no CPU fallback)") from e
+    from specb200.build import torch_ops_target
+
+    if _torch_ops.target != torch_ops_target():
+        raise RuntimeError(f"specb200/_torch_ops.so was built for {_torch_ops.target}, not {torch_ops_target()}: build it "
+                           "again with `python -m specb200.build`")
     return _torch_ops
 
 

@@ -60,25 +60,46 @@ def _run(cmd: list[str], what: str, verbose: bool) -> None:
         raise RuntimeError(f"{what} failed:\n{res.stdout}\n{res.stderr}")
 
 
+def torch_ops_target() -> str:
+    """What the extension module is compiled for: it uses torch's C++ classes and Python's C API."""
+    import torch
+
+    return (f"torch {torch.__version__}, C++11 ABI {int(torch._C._GLIBCXX_USE_CXX11_ABI)}, "
+            f"Python {sys.version_info.major}.{sys.version_info.minor}")
+
+
+def _torch_ops_up_to_date() -> bool:
+    stamp = TORCH_OPS.with_suffix(".stamp")
+    if not TORCH_OPS.exists() or not stamp.exists() or stamp.read_text() != torch_ops_target():
+        return False
+    built = TORCH_OPS.stat().st_mtime
+    return all(p.stat().st_mtime <= built for p in (TORCH_OPS_SRC, INCLUDE / "specb200.h"))
+
+
 def build_torch_ops(verbose: bool = False, force: bool = False) -> Path:
-    """The extension module, linked to libspecb200.so beside it and to the installed torch."""
-    inputs = [TORCH_OPS_SRC, INCLUDE / "specb200.h"]
-    if not force and TORCH_OPS.exists() and all(p.stat().st_mtime <= TORCH_OPS.stat().st_mtime for p in inputs):
+    """The extension module, linked to libspecb200.so beside it and to the installed torch. A stamp beside it
+    says what it was built for, so that another torch or Python builds it again."""
+    if not force and _torch_ops_up_to_date():
         return TORCH_OPS
     import sysconfig
 
     import torch
 
+    gxx = shutil.which("g++")
+    if gxx is None:
+        raise RuntimeError("g++ not found: the 8-bit operators of specb200.ops need _torch_ops.so (libspecb200.so is built)")
     base = Path(torch.__file__).resolve().parent
     cuda = Path(nvcc()).resolve().parents[1]
     tmp = TORCH_OPS.with_suffix(".so.tmp")
-    _run([shutil.which("g++") or "g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
-          f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+    _run([gxx, "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
+          f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f'-DSPECB200_TARGET="{torch_ops_target()}"',
           *(f"-I{p}" for p in (INCLUDE, sysconfig.get_paths()["include"], cuda / "include")),
           *(f"-isystem{p}" for p in (base / "include", base / "include" / "torch" / "csrc" / "api" / "include")),
           str(TORCH_OPS_SRC), "-o", str(tmp), f"-L{PKG}", "-l:libspecb200.so", f"-L{base / 'lib'}", "-lc10", "-lc10_cuda",
-          "-ltorch_cpu", "-ltorch", "-ltorch_python", "-Wl,-rpath,$ORIGIN"], "_torch_ops", verbose)
+          "-ltorch_cpu", "-ltorch", "-ltorch_python", "-Wl,-rpath,$ORIGIN"], "_torch_ops (the 8-bit operators of specb200.ops; libspecb200.so is built)",
+         verbose)
     os.replace(tmp, TORCH_OPS)
+    TORCH_OPS.with_suffix(".stamp").write_text(torch_ops_target())
     return TORCH_OPS
 
 

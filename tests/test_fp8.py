@@ -179,6 +179,37 @@ def test_host_tensors_are_refused():
             call(_ops())
 
 
+def test_the_extension_module_is_built_again_for_another_torch(monkeypatch, tmp_path):
+    """It uses torch's C++ classes: one that was built for another torch is neither taken for up to date nor loaded."""
+    from specb200 import _ffi, build
+
+    runs = []
+
+    def run(cmd, what, verbose):
+        runs.append(cmd)
+        build.Path(cmd[cmd.index("-o") + 1]).write_bytes(b"built")
+
+    monkeypatch.setattr(build, "_run", run)
+    monkeypatch.setattr(build, "TORCH_OPS", tmp_path / "_torch_ops.so")
+    for want in (1, 1):
+        build.build_torch_ops()
+        assert len(runs) == want
+    (tmp_path / "_torch_ops.stamp").unlink()  # a module of unknown origin
+    build.build_torch_ops()
+    assert len(runs) == 2
+    module = _ffi.torch_ops()
+    assert module.target == build.torch_ops_target()
+    monkeypatch.setattr(torch, "__version__", "2.99.0")
+    build.build_torch_ops()
+    build.build_torch_ops()
+    assert len(runs) == 3 and any("2.99.0" in arg for arg in runs[-1])
+    with pytest.raises(RuntimeError, match="build it again"):
+        _ffi.torch_ops()
+    monkeypatch.setattr(build.shutil, "which", lambda name: None)
+    with pytest.raises(RuntimeError, match="g\\+\\+ not found"):
+        build.build_torch_ops(force=True)
+
+
 @pytest.mark.gpu
 def test_wrappers_refuse_mismatched_tensors():
     ops = _ops()
