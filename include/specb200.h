@@ -270,8 +270,8 @@ int specb200_attention(int dtype, const void* q, const void* k_pool, const void*
  *   s = max(max |y| over the group, 2^-100) / 448,   q = e4m3(y / s), nearest even.
  * Activations [M, K] have a scale per row and 128 columns: scales [M, ceil(K / 128)] fp32.
  * Weights [N, K] have one per 128 x 128 block: [ceil(N / 128), ceil(K / 128)]. The last groups
- * may be short. Row pitches (ld*) count elements; any pitch and alignment is accepted except
- * where a function says otherwise, rows on 16-byte boundaries are faster (from others whole 16-byte
+ * may be short. Row pitches (ld*) count elements; any pitch and any start on a boundary of the
+ * elements is accepted except where a function says otherwise, rows on 16-byte boundaries are faster (from others whole 16-byte
  * units are read, so what lies between two rows may be read, but nothing before the first row or
  * behind the last). A NaN in a group
  * makes its values and scale NaN, an infinity makes the scale infinite. Nothing is written

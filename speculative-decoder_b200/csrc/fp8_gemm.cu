@@ -1224,6 +1224,8 @@ int run_linear_fp8(const void* x, int64_t ldx, const float* x_scales, const void
   if (!x || !x_scales || !w || !w_scales || !y) return specb200_set_error(SPECB200_ERR_ARG, "linear_fp8: null pointer");
   if (!fp8_aligned(x, 16) || !fp8_aligned(w, 16))
     return specb200_set_error(SPECB200_ERR_ARG, "linear_fp8: operands must start on 16-byte boundaries");
+  if (!fp8_aligned(x_scales, 4) || !fp8_aligned(w_scales, 4) || !fp8_aligned(y, out_f32 ? 4 : 2) || !fp8_aligned(status, 4))
+    return specb200_set_error(SPECB200_ERR_ARG, "linear_fp8: a pointer is not on a boundary of its elements");
   const F8Plan p = plan_fp8(M, N, K);
   if (static_cast<int64_t>(p.m_tiles) * p.n_tiles > (1 << 30)) return specb200_set_error(SPECB200_ERR_ARG, "linear_fp8: M x N too large");
   CUtensorMap wm, xm;

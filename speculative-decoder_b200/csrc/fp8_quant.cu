@@ -746,6 +746,7 @@ int finish(cudaError_t e) {
   return e == cudaSuccess ? SPECB200_OK : specb200_set_error(SPECB200_ERR_CUDA, cudaGetErrorString(e));
 }
 // 2^31 - 1 CTAs of 16 groups each, and the pitches in range
+uint64_t bytes_of(int dtype) { return dtype == SPECB200_BF16 ? 2 : 4; }
 bool sizes_ok(int M, int K) { return M >= 0 && K > 0 && K <= (1 << 30) && (static_cast<int64_t>(M) * groups_of(K) + 15) / 16 <= 0x7fffffff; }
 }  // namespace
 
@@ -758,6 +759,8 @@ extern "C" int specb200_quantize_fp8(int dtype, const void* x, int64_t ldx, int 
   if (dtype != SPECB200_F32 && dtype != SPECB200_BF16) return specb200_set_error(SPECB200_ERR_UNSUPPORTED, "quantize_fp8: dtype");
   if (M == 0) return SPECB200_OK;
   if (!x || !q || !scales) return specb200_set_error(SPECB200_ERR_ARG, "quantize_fp8: null pointer");
+  if (!fp8_aligned(x, bytes_of(dtype)) || !fp8_aligned(scales, 4))
+    return specb200_set_error(SPECB200_ERR_ARG, "quantize_fp8: a pointer is not on a boundary of its elements");
   RowArgs a = {};
   a.x = x;
   a.ldx = ldx;
@@ -780,6 +783,8 @@ extern "C" int specb200_silu_mul_fp8(int dtype, const void* gate_up, int64_t ld,
   if (dtype != SPECB200_F32 && dtype != SPECB200_BF16) return specb200_set_error(SPECB200_ERR_UNSUPPORTED, "silu_mul_fp8: dtype");
   if (M == 0) return SPECB200_OK;
   if (!gate_up || !q || !scales) return specb200_set_error(SPECB200_ERR_ARG, "silu_mul_fp8: null pointer");
+  if (!fp8_aligned(gate_up, bytes_of(dtype)) || !fp8_aligned(scales, 4))
+    return specb200_set_error(SPECB200_ERR_ARG, "silu_mul_fp8: a pointer is not on a boundary of its elements");
   RowArgs a = {};
   a.x = gate_up;
   a.ldx = ld;
@@ -804,6 +809,11 @@ extern "C" int specb200_rmsnorm_fp8(int dtype, const void* x, int64_t ldx, const
   if (H > kNormMaxWidth) return specb200_set_error(SPECB200_ERR_UNSUPPORTED, "rmsnorm_fp8: H is at most 32768");
   if (M == 0) return SPECB200_OK;
   if (!x || !weight || !q || !scales || (delta && !h)) return specb200_set_error(SPECB200_ERR_ARG, "rmsnorm_fp8: null pointer");
+  const uint64_t e = bytes_of(dtype);
+  if (!fp8_aligned(x, e) || !fp8_aligned(weight, e) || !fp8_aligned(delta, e) || (delta && !fp8_aligned(h, e)) || !fp8_aligned(scales, 4))
+    return specb200_set_error(SPECB200_ERR_ARG, "rmsnorm_fp8: a pointer is not on a boundary of its elements");
+  if (delta && ((h == x && ldh != ldx) || (h == delta && ldh != ldd)))
+    return specb200_set_error(SPECB200_ERR_ARG, "rmsnorm_fp8: h in the place of x or delta has its row pitch");
   NormArgs a = {};
   a.x = x;
   a.ldx = ldx;

@@ -171,6 +171,44 @@ def test_linear_refuses_bad_arguments_on_the_host():
     assert call(M=0) == _ffi.OK
 
 
+def test_pointers_off_their_elements_are_refused_on_the_host():
+    """Kernels read single elements at the ends of rows: a pointer between two of them would be a misaligned access."""
+    from specb200 import _ffi
+
+    lib = _lib()
+    keep, p = _buf()
+
+    def refused(call, ok, **bad):
+        assert call(*{**ok, **bad}.values(), None) == _ffi.ERR_ARG, bad
+        assert b"boundary of its elements" in lib.specb200_last_error(), bad
+
+    for dtype, off in ((_ffi.BF16, 1), (_ffi.F32, 2)):
+        ok = dict(dtype=dtype, x=p, ldx=64, M=2, K=64, rows=1, q=p, ldq=64, s=p)
+        for bad in (dict(x=p + off), dict(s=p + 2)):
+            refused(lib.specb200_quantize_fp8, ok, **bad)
+            refused(lib.specb200_quantize_fp8, ok, rows=128, **bad)
+        ok = dict(dtype=dtype, x=p, ldx=64, d=p, ldd=64, w=p, M=2, H=64, eps=1e-5, h=p, ldh=64, q=p, ldq=64, s=p)
+        for bad in (dict(x=p + off), dict(d=p + off), dict(w=p + off), dict(h=p + off), dict(s=p + 1)):
+            refused(lib.specb200_rmsnorm_fp8, ok, **bad)
+        ok = dict(dtype=dtype, x=p, ld=128, M=2, I=64, packed=0, q=p, ldq=64, s=p)
+        for bad in (dict(x=p + off), dict(s=p + 2)):
+            refused(lib.specb200_silu_mul_fp8, ok, **bad)
+    ok = dict(x=p, ldx=64, xs=p, w=p, ldw=64, ws=p, M=2, N=16, K=64, f32=0, y=p, ldy=16, status=None)
+    for bad in (dict(xs=p + 2), dict(ws=p + 1), dict(y=p + 1), dict(f32=1, y=p + 2), dict(status=p + 2)):
+        refused(lib.specb200_linear_fp8, ok, **bad)
+
+
+def test_a_residual_in_place_has_its_own_pitch():
+    from specb200 import _ffi
+
+    lib = _lib()
+    keep, p = _buf()
+    ok = dict(dtype=_ffi.BF16, x=p, ldx=64, d=p + 256, ldd=72, w=p, M=2, H=64, eps=1e-5, h=p, ldh=72, q=p, ldq=64, s=p)
+    for change in ({}, dict(h=p + 256, ldh=64)):
+        assert lib.specb200_rmsnorm_fp8(*{**ok, **change}.values(), None) == _ffi.ERR_ARG
+        assert b"row pitch" in lib.specb200_last_error()
+
+
 def test_host_tensors_are_refused():
     x = torch.zeros(2, 64)
     for call in (lambda o: o.quantize_fp8(x), lambda o: o.rmsnorm_fp8(x, x[0], 1e-5), lambda o: o.silu_mul_fp8(x),
