@@ -38,7 +38,10 @@ std::string shape(const at::Tensor& t) { return text(t.sizes()); }
 
 const at::Tensor& tensor(PyObject* o, const char* where) {
   if (!THPVariable_Check(o)) throw Refusal{PyExc_TypeError, text(where, ": expected a tensor, got ", Py_TYPE(o)->tp_name)};
-  return THPVariable_Unpack(o);
+  const at::Tensor& t = THPVariable_Unpack(o);
+  // such a view's memory holds the values with the other sign
+  if (t.is_neg()) bad(text(where, ": a view that is negated on reading (call resolve_neg() first)"));
+  return t;
 }
 bool truth(PyObject* o) {
   const int v = PyObject_IsTrue(o);

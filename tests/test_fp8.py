@@ -248,6 +248,16 @@ def test_the_extension_module_is_built_again_for_another_torch(monkeypatch, tmp_
         build.build_torch_ops(force=True)
 
 
+def test_negated_views_are_refused():
+    """The imaginary part of a conjugate holds its values with the other sign in memory."""
+    x, neg = torch.zeros(2, 64), torch.zeros(2, 1, dtype=torch.complex64).conj().imag
+    for call in (lambda o: o.quantize_fp8(neg), lambda o: o.rmsnorm_fp8(neg, neg[0], 1e-5),
+                 lambda o: o.rmsnorm_fp8(x, x[0], 1e-5, delta=neg), lambda o: o.silu_mul_fp8(neg),
+                 lambda o: o.linear_fp8(x.to(F8), neg, x.to(F8), x)):
+        with pytest.raises(ValueError, match="resolve_neg"):
+            call(_ops())
+
+
 @pytest.mark.gpu
 def test_wrappers_refuse_mismatched_tensors():
     ops = _ops()
