@@ -529,6 +529,34 @@ def test_rmsnorm_of_views_and_in_place(dtype):
     assert rc == 0 and torch.equal(x, h) and torch.equal(s2, s) and torch.equal(q2, q.contiguous().view(torch.uint8))
 
 
+# more rows than the grid takes at once, with a ragged last round: loads ahead (one group per octet), several rows
+# per CTA on and off the 16-byte boundaries (teams that meet inside a warp), two and four groups per octet
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("m,k", [(5000, 2048), (14001, 576), (9001, 129), (20001, 301), (1500, 4104), (1300, 4105), (700, 8201),
+                                 (3, 8201), (2, 32767), (40000, 64)])
+def test_rmsnorm_walks_over_its_rows(m, k, dtype):
+    from specb200 import _ffi
+
+    ops, lib = _ops(), _lib()
+    x, d = _rand(m + k, m, k, dtype=dtype), _rand(m + k + 1, m, k, dtype=dtype)
+    weight = (1 + 0.3 * _rand(k, k, spread=0.0)).to(dtype)
+    q, s = ops.rmsnorm_fp8(x, weight, 1e-5)
+    _check_quantized(q, s, _norm64(x, weight, 1e-5), d=4 * U, s_tol=NORM_S)
+    q, s, h = ops.rmsnorm_fp8(x, weight, 1e-5, delta=d)
+    assert torch.equal(h, (x.float() + d.float()).to(dtype))
+    _check_quantized(q, s, _norm64(h, weight, 1e-5), d=4 * U, s_tol=NORM_S)
+    # the same in the place of x and of delta, through the C ABI and into dense rows
+    for place in (0, 1):
+        x2, d2 = x.clone(), d.clone()
+        h2 = d2 if place else x2
+        q2, s2 = torch.empty(m, k, dtype=torch.uint8, device=DEV), torch.empty_like(s)
+        rc = lib.specb200_rmsnorm_fp8(_ffi.BF16 if dtype == BF16 else _ffi.F32, x2.data_ptr(), k, d2.data_ptr(), k,
+                                      weight.data_ptr(), m, k, 1e-5, h2.data_ptr(), k, q2.data_ptr(), k, s2.data_ptr(),
+                                      torch.cuda.current_stream().cuda_stream)
+        assert rc == 0 and torch.equal(h2, h) and torch.equal(s2, s) and torch.equal(q2.view(F8).float(), q.float())
+
+
 @pytest.mark.gpu
 def test_rmsnorm_edge_rows():
     """A row of zeros, rows so small that eps decides, groups under the floor, weights of zero, and
@@ -819,6 +847,21 @@ def test_linear_repeats_bit_for_bit(m, n, k):
     _check_product(first, x, xs, w, ws, True)
     again = [ops.linear_fp8(x, xs, w, ws, out_f32=True, check=False) for _ in range(30)]
     assert all(torch.equal(y, first) for y in again)
+
+
+# products of two CTAs per SM whose groups go round the ring of stages, the scales' slots and the TMEM buffers
+# several times: up to 16 tokens and more, odd numbers of groups, a short last group, a short last tile
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", [(16, 25600, 2048), (5, 20000, 1160), (1, 19001, 4999), (24, 25600, 2048),
+                                   (100, 19100, 1160), (128, 25600, 1024), (33, 19201, 2900)])
+def test_linear_on_shared_sms_goes_round_its_rings(m, n, k):
+    ops = _ops()
+    x, xs, w, ws = _operands(m + n + k, m, n, k)
+    first = ops.linear_fp8(x, xs, w, ws, out_f32=True)
+    _check_product(first, x, xs, w, ws, True)
+    again = [ops.linear_fp8(x, xs, w, ws, out_f32=True, check=False) for _ in range(10)]
+    assert all(torch.equal(y, first) for y in again)
+    assert torch.equal(ops.linear_fp8(x, xs, w, ws), first.bfloat16())
 
 
 @pytest.mark.gpu
