@@ -276,9 +276,9 @@ SPECB200_DEVINL void tma_store_2d(const CUtensorMap* map, const void* smem_src, 
                : "memory");
 }
 
-// NaN for what a warp could not finish because a wait gave up, so that the caller sees it without a status word
-// too: up to 32 tokens of its features, and in a cluster's partial tile what the splits add up. (NaN in the
-// sums on the way of the ordinary stores cost every call of the small kernel 0.15 us.)
+// NaN for 32 tokens of a warp's features that it could not finish because a wait gave up, so that the caller sees
+// it without a status word too. (NaN in the sums on the way of the ordinary stores cost every call of the
+// small kernel 0.15 us.)
 constexpr uint32_t kF8Nan = 0x7fffffffu;
 SPECB200_DEVINL void give_up_outputs(const F8Args& a, int m0, int n0, int cols, int lane) {
   const int rows = min(32, a.M - m0), end = min(n0 + cols, a.N);
@@ -929,13 +929,13 @@ __global__ void __launch_bounds__(kF8PairThreads, 1)
       const int64_t pitch = static_cast<int64_t>(32) * kblocks;
       uint32_t st = 0, phase = 0, slot = 0, last = 0, last_phase = 0;
       bool ok = true, mine = !odd, any = false;
-      for (F8TileWalk tile(a); tile.more() && ok; tile.next()) {
+      for (F8TileWalk tile(a); tile.more() && ok && !a.starved; tile.next()) {
         const int m0 = tile.token0(rank), n0 = tile.feature0(), block = 2 * tile.n + lane;
         const float* sx = a.xs + static_cast<int64_t>(m0 + lane) * kblocks;
         const float* sw = a.ws + static_cast<int64_t>(block) * kblocks;
         const bool live_w = lane < 2 && block * kF8Block < a.N;
         for (int kb = 0; kb < kblocks; ++kb, mine = !mine) {
-          if (mine && !a.starved) {
+          if (mine) {
             ok = wait_warp(&bars.done[1][st], phase ^ 1, a.status, &abort_flag);
             if (!ok) break;
             if (lane == 0) {
@@ -1019,8 +1019,7 @@ __global__ void __launch_bounds__(kF8PairThreads, 1)
       return __all_sync(0xffffffffu, tried) || wait_warp(&bars.done[1][st], phase, a.status, &abort_flag);
     };
     auto factor = [&] { return bars.scales[slot].x[quarter * 32 + lane] * bars.scales[slot].w[block]; };
-    F8TileWalk tile(a);
-    for (; tile.more() && ok; tile.next()) {
+    for (F8TileWalk tile(a); tile.more() && ok; tile.next()) {
       const int m0 = tile.token0(rank) + quarter * 32, n0 = tile.feature0() + block * kF8Block;
       if (m0 >= a.M || n0 >= a.N) {  // a warp without outputs only keeps step
         for (int kb = 0; kb < kblocks; ++kb) {
@@ -1085,14 +1084,22 @@ __global__ void __launch_bounds__(kF8PairThreads, 1)
       else
         store_warp_tile<__nv_bfloat16, kF8PairPieces>(a, y_map, acc, out_buf, m0, n0, lane);
     }
-    for (; tile.more() && !ok; tile.next())
-      give_up_outputs(a, tile.token0(rank) + quarter * 32, tile.feature0() + block * kF8Block, kCols, lane);
     if (a.rows16 && lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
     __syncwarp();
   }
   tc_fence_before();
   cluster_arrive_wait();  // every arrival at the other's barriers has landed
   __syncthreads();
+  // NaN over the tiles of a CTA in which a wait gave up. Here, with nothing kept for it through the loops, whose
+  // registers are spent (8192 x 16384 x 2048: 248 us with it where the epilogue's loop ends, 245 without).
+  if (__builtin_expect(*reinterpret_cast<volatile int*>(&abort_flag), 0)) {
+    int t, r;
+    asm volatile("mov.u32 %0, %%tid.x;" : "=r"(t));
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    if (t < kF8EpiWarps * 32)
+      for (F8TileWalk tile(a); tile.more(); tile.next())
+        give_up_outputs(a, tile.token0(r) + (t >> 5 & 3) * 32, tile.feature0() + (t >> 7) * kF8Block, kF8Block, t & 31);
+  }
   if (warp == 9) {
     tc_fence_after();
     f8_tmem_dealloc<true>(tmem, 512);
