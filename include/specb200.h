@@ -288,7 +288,7 @@ int specb200_quantize_fp8(int dtype, const void* x, int64_t ldx, int M, int K, i
 
 /* RMSNorm with the residual update in front and an 8-bit output:
  *   h = T(x + delta) (delta NULL: h = x, not stored; h may be x or delta, with its pitch),
- *   y = weight * h / sqrt(mean(h^2) + eps) in fp32, (q, scales) = quantized y.
+ *   y = weight * h / sqrt(mean(h^2) + eps) in fp32 (weight * h first), (q, scales) = quantized y.
  * H <= 32768 (SPECB200_ERR_UNSUPPORTED beyond). */
 int specb200_rmsnorm_fp8(int dtype, const void* x, int64_t ldx, const void* delta, int64_t ldd, const void* weight,
                          int M, int H, float eps, void* h, int64_t ldh, void* q, int64_t ldq, float* scales,

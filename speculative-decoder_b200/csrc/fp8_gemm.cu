@@ -1034,8 +1034,8 @@ __global__ void __launch_bounds__(kF8PairThreads, 1)
       f32x2 acc2[kCols / 2];
 #pragma unroll
       for (int i = 0; i < kCols / 2; ++i) acc2[i] = 0;
-      // 32 columns come back at a time, the next ones and the next poll on their way while the last
-      // ones are added.
+      // A half's 64 columns come back in two reads and are added once both are there, with the poll for the next
+      // half on its way; no read is.
       uint32_t r0[kLd], r1[kLd];
       auto add = [&](int c, const uint32_t (&r)[kLd], float f) {
 #pragma unroll
