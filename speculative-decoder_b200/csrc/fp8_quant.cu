@@ -812,7 +812,7 @@ extern "C" int specb200_rmsnorm_fp8(int dtype, const void* x, int64_t ldx, const
   const uint64_t e = bytes_of(dtype);
   if (!fp8_aligned(x, e) || !fp8_aligned(weight, e) || !fp8_aligned(delta, e) || (delta && !fp8_aligned(h, e)) || !fp8_aligned(scales, 4))
     return specb200_set_error(SPECB200_ERR_ARG, "rmsnorm_fp8: a pointer is not on a boundary of its elements");
-  if (delta && ((h == x && ldh != ldx) || (h == delta && ldh != ldd)))
+  if (delta && M > 1 && ((h == x && ldh != ldx) || (h == delta && ldh != ldd)))
     return specb200_set_error(SPECB200_ERR_ARG, "rmsnorm_fp8: h in the place of x or delta has its row pitch");
   NormArgs a = {};
   a.x = x;

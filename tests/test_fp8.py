@@ -558,6 +558,18 @@ def test_rmsnorm_walks_over_its_rows(m, k, dtype):
 
 
 @pytest.mark.gpu
+def test_one_row_in_place_with_any_pitch():
+    from specb200 import _ffi
+
+    x, d, weight = (_rand(i, 64, dtype=BF16) for i in (20, 21, 22))
+    want = _ops().rmsnorm_fp8(x, weight, 1e-5, delta=d)
+    q, s = torch.empty(64, dtype=torch.uint8, device=DEV), torch.empty_like(want[1])
+    rc = _lib().specb200_rmsnorm_fp8(_ffi.BF16, x.data_ptr(), 64, d.data_ptr(), 72, weight.data_ptr(), 1, 64, 1e-5,
+                                     x.data_ptr(), 100, q.data_ptr(), 64, s.data_ptr(), torch.cuda.current_stream().cuda_stream)
+    assert rc == 0 and torch.equal(x, want[2]) and torch.equal(s, want[1]) and torch.equal(q.view(F8).float(), want[0].float())
+
+
+@pytest.mark.gpu
 def test_rmsnorm_edge_rows():
     """A row of zeros, rows so small that eps decides, groups under the floor, weights of zero, and
     rows that hold a NaN or an infinity: each keeps to itself."""
