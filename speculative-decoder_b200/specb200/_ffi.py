@@ -122,9 +122,10 @@ def torch_ops():
                            "(the engine has no CPU fallback)") from e
     from specb200.build import torch_ops_target
 
-    if _torch_ops.target != torch_ops_target():
-        raise RuntimeError(f"specb200/_torch_ops.so was built for {_torch_ops.target}, not {torch_ops_target()}: build it "
-                           "again with `python -m specb200.build`")
+    target = getattr(_torch_ops, "target", "an unknown torch")
+    if target != torch_ops_target():
+        raise RuntimeError(f"specb200/_torch_ops.so was built for {target}, not {torch_ops_target()}: build it again with "
+                           "`python -m specb200.build`")
     return _torch_ops
 
 

@@ -243,6 +243,9 @@ def test_the_extension_module_is_built_again_for_another_torch(monkeypatch, tmp_
     assert len(runs) == 3 and any("2.99.0" in arg for arg in runs[-1])
     with pytest.raises(RuntimeError, match="build it again"):
         _ffi.torch_ops()
+    monkeypatch.delattr(module, "target")  # a module from before it said so
+    with pytest.raises(RuntimeError, match="unknown torch"):
+        _ffi.torch_ops()
     monkeypatch.setattr(build.shutil, "which", lambda name: None)
     with pytest.raises(RuntimeError, match="g\\+\\+ not found"):
         build.build_torch_ops(force=True)
